@@ -341,6 +341,140 @@ int jb_merge_topk_strided(const int32_t* shard_idx, const float* shard_dist, uin
                           uint32_t n_shards, uint64_t n_queries, uint32_t k, int32_t* out_idx,
                           float* out_dist, void* stream);
 
+/* ── paged key-value cache ───────────────────────────────────────────── */
+/* What a language model that reads the passages of a search needs next: its
+ * key-value cache in pages, so that the ids of a search's answer can stand as
+ * a page table.  No reference counterpart.  All pointers are device pointers
+ * and all calls are asynchronous on `stream` and, given device-resident
+ * arguments only, can be captured into a CUDA graph. */
+
+#define JB_F16 0
+#define JB_BF16 1
+#define JB_F32 2
+
+/* Bits that the kernels set in a cache's status word (never cleared by them):
+ * a row that needs a page found none free; a row of a call is out of range,
+ * named twice, too long for its table or not empty where it has to be; a
+ * token's place, or a page's number, is out of range. */
+#define JB_PAGES_EXHAUSTED 1
+#define JB_PAGES_BAD_ROW 2
+#define JB_PAGES_BAD_TOKEN 4
+
+/* Keys and values are [n_layers][n_pages][page_size][n_kv_heads][head_dim]
+ * elements of `dtype` (JB_F16 or JB_BF16) at the given strides (in elements,
+ * the same for both; head_dim contiguous; every stride, and both bases, a
+ * multiple of 16 bytes; head_dim a multiple of 8, at most 256).  A row (a
+ * conversation) holds lengths[row] tokens in the pages table[row][0 ..
+ * ceil(length / page_size)); an entry of -1 is a page that is not there: its
+ * tokens are never attended to.  refs[page] counts the rows that hold a page;
+ * 0 is free. */
+typedef struct jb_page_cache {
+  void* k;
+  void* v;
+  int32_t* table;   /* [n_rows][max_pages], rows table_stride entries apart */
+  int32_t* lengths; /* [n_rows] */
+  int32_t* refs;    /* [n_pages] */
+  int32_t* status;  /* one word of JB_PAGES_* bits */
+  int64_t layer_stride, page_stride, token_stride, head_stride;
+  int64_t table_stride;
+  uint32_t n_layers, n_pages, page_size, n_kv_heads, head_dim;
+  uint32_t n_rows, max_pages;
+  int32_t dtype;
+  int32_t device;
+} jb_page_cache;
+
+/* Rotary positions: y = x with the first rot_dim elements of each head turned
+ * by the token's position, times `scale`; the rest is copied.  Pairs are
+ * (i, i + rot_dim / 2), or (2i, 2i + 1) with `interleaved`.  freq[i] (device,
+ * rot_dim / 2 values) is pair i's turn for one position in units of 2^-64 of
+ * a turn: products with whole positions wrap at whole turns, so angles are
+ * exact to float32 for every int64 position.  `inverse` turns backwards: the
+ * gradient with respect to x, given y's.  x and y: [n_tokens][n_heads]
+ * [head_dim] of `dtype` at any token and head stride (elements); y may be x.
+ * positions: n_tokens int32, or int64 with positions_64.  Runs on the current
+ * device. */
+int jb_rotary(const void* x, int64_t x_token_stride, int64_t x_head_stride, void* y,
+              int64_t y_token_stride, int64_t y_head_stride, int32_t dtype, uint64_t n_tokens,
+              uint32_t n_heads, uint32_t head_dim, uint32_t rot_dim, const void* positions,
+              int32_t positions_64, const int64_t* freq, float scale, int32_t interleaved,
+              int32_t inverse, void* stream);
+
+/* Writes n_tokens new keys and values ([n_tokens][n_kv_heads][head_dim] of the
+ * cache's type, any token and head stride) into one layer: token t becomes
+ * token index[t] of row rows[t] (index NULL: the row's last, lengths[row] -
+ * 1).  With freq, keys are rotated on the way as by jb_rotary (positions NULL:
+ * the token's index), and with q so are n_q_heads query heads, into q_out
+ * (which may be q).  The page must not be shared with a row that still needs
+ * its old tokens there (jb_pages_fork sees to that).  A token whose place
+ * does not exist is not written and sets JB_PAGES_BAD_TOKEN.  No two tokens
+ * may have the same place. */
+int jb_kv_append(const jb_page_cache* cache, uint32_t layer, uint64_t n_tokens, const void* q,
+                 int64_t q_token_stride, int64_t q_head_stride, void* q_out,
+                 int64_t q_out_token_stride, int64_t q_out_head_stride, uint32_t n_q_heads,
+                 const void* k, int64_t k_token_stride, int64_t k_head_stride, const void* v,
+                 int64_t v_token_stride, int64_t v_head_stride, const int32_t* rows,
+                 const int32_t* index, const void* positions, int32_t positions_64,
+                 const int64_t* freq, uint32_t rot_dim, float scale, int32_t interleaved,
+                 void* stream);
+
+/* Gives row rows[i] room for tokens[i] more tokens: new pages where its last
+ * one is full (the free pages with the lowest numbers, in the order of the
+ * rows), and a length that counts them.  Rows are served in order until the
+ * free pages run out; from the first that finds too few on, rows that need
+ * pages are left as they were (JB_PAGES_EXHAUSTED). */
+int jb_pages_extend(const jb_page_cache* cache, const int32_t* rows, const int32_t* tokens,
+                    uint32_t n, void* stream);
+
+/* Makes the empty row children[i] a copy of row parents[i] as it was at the
+ * call: whole pages are shared, a page that is filled in part is copied (its
+ * tokens in every layer, into the lowest free page), so that each can append
+ * on its own.  Pairs are served in order as in jb_pages_extend. */
+int jb_pages_fork(const jb_page_cache* cache, const int32_t* parents, const int32_t* children,
+                  uint32_t n, void* stream);
+
+/* Empties rows: each of their pages loses a holder, and is free when it was
+ * the last.  A row that is empty already, or named twice, is no error. */
+int jb_pages_free(const jb_page_cache* cache, const int32_t* rows, uint32_t n, void* stream);
+
+/* Gives the empty row rows[i] the first ceil(lengths[i] / page_size) of the m
+ * pages at pages + i * pages_stride as further holder (a search's ids, or
+ * another row's pages; -1 and, with JB_PAGES_BAD_TOKEN, numbers out of range
+ * stand for pages that are not there).  lengths NULL: m whole pages each. */
+int jb_pages_adopt(const jb_page_cache* cache, const int32_t* rows, const int32_t* pages,
+                   int64_t pages_stride, uint32_t m, const int32_t* lengths, uint32_t n,
+                   void* stream);
+
+/* Moves the live pages together: with L live pages, the j-th live page
+ * numbered L or above moves to the j-th free number below L, in keys, values,
+ * refs and every row's table.  remap[p] is page p's new number, -1 if it was
+ * free (n_pages int32). */
+int jb_pages_compact(const jb_page_cache* cache, int32_t* remap, void* stream);
+
+/* Copies keys and values of page src[i] to page dst[i], in every layer.  No
+ * page may be among dst twice, or among both.  Pairs with a number out of
+ * range are left out (JB_PAGES_BAD_TOKEN). */
+int jb_pages_copy(const jb_page_cache* cache, const int32_t* src, const int32_t* dst, uint32_t n,
+                  void* stream);
+
+/* Attention of one new token of each of n rows over the row's tokens in one
+ * layer: out = sum_t p_t v_t with p = softmax(scale * q . k_t), for
+ * n_q_heads query heads, n_q_heads / n_kv_heads of them to each key-value
+ * head in turn.  Query i reads row rows[i] (NULL: row i; a row out of range
+ * has no tokens).  Tokens that are not attended to: those of pages that are
+ * not there, those t < mask_width with mask[i * mask_stride + t] = 0 (bytes;
+ * NULL: none), and with window > 0 all but the row's last `window`.  What
+ * their keys and values hold does not matter.  q and out: [n][n_q_heads][head_dim] of the
+ * cache's type at any stride that is a multiple of 16 bytes.  lse (float32
+ * [n][n_q_heads], or NULL): log sum exp of the scaled scores, with which parts
+ * of one attention can be joined.  A query with nothing to attend to gives
+ * zeros, and lse -inf. */
+int jb_paged_attention(const jb_page_cache* cache, uint32_t layer, const void* q,
+                       int64_t q_row_stride, int64_t q_head_stride, void* out,
+                       int64_t out_row_stride, int64_t out_head_stride, uint32_t n,
+                       uint32_t n_q_heads, const int32_t* rows, const uint8_t* mask,
+                       int64_t mask_stride, uint32_t mask_width, uint32_t window, float scale,
+                       float* lse, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

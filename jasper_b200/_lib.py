@@ -35,7 +35,21 @@ class GraphInfo(C.Structure):
     ]
 
 
+class PageCache(C.Structure):
+    """jb_page_cache."""
+    _fields_ = [
+        ("k", C.c_void_p), ("v", C.c_void_p), ("table", C.c_void_p), ("lengths", C.c_void_p),
+        ("refs", C.c_void_p), ("status", C.c_void_p),
+        ("layer_stride", C.c_int64), ("page_stride", C.c_int64), ("token_stride", C.c_int64),
+        ("head_stride", C.c_int64), ("table_stride", C.c_int64),
+        ("n_layers", C.c_uint32), ("n_pages", C.c_uint32), ("page_size", C.c_uint32),
+        ("n_kv_heads", C.c_uint32), ("head_dim", C.c_uint32), ("n_rows", C.c_uint32),
+        ("max_pages", C.c_uint32), ("dtype", C.c_int32), ("device", C.c_int32),
+    ]
+
+
 _P = C.c_void_p
+_F32 = C.c_float
 _U32, _U64, _I32, _I64 = C.c_uint32, C.c_uint64, C.c_int32, C.c_int64
 
 # name -> argument types (all return int status)
@@ -82,6 +96,18 @@ SIGNATURES: dict[str, list] = {
     "jb_graph_get_rabitq": [_I64, C.POINTER(_U32), _P, _P],
     "jb_graph_search_rabitq": [_I64, _P, _U64, _U32, _P, _P, _U32, _U32, _U32, C.c_float, _P, _P],
     "jb_graph_get_rabitq_err": [_I64, _P],
+    "jb_rotary": [_P, _I64, _I64, _P, _I64, _I64, _I32, _U64, _U32, _U32, _U32, _P, _I32, _P, _F32,
+                  _I32, _I32, _P],
+    "jb_kv_append": [_P, _U32, _U64, _P, _I64, _I64, _P, _I64, _I64, _U32, _P, _I64, _I64, _P,
+                     _I64, _I64, _P, _P, _P, _I32, _P, _U32, _F32, _I32, _P],
+    "jb_pages_extend": [_P, _P, _P, _U32, _P],
+    "jb_pages_fork": [_P, _P, _P, _U32, _P],
+    "jb_pages_free": [_P, _P, _U32, _P],
+    "jb_pages_adopt": [_P, _P, _P, _I64, _U32, _P, _U32, _P],
+    "jb_pages_compact": [_P, _P, _P],
+    "jb_pages_copy": [_P, _P, _P, _U32, _P],
+    "jb_paged_attention": [_P, _U32, _P, _I64, _I64, _P, _I64, _I64, _U32, _U32, _P, _P, _I64,
+                           _U32, _U32, _F32, _P, _P],
 }
 
 

@@ -233,9 +233,10 @@ void search_impl(const jb::Graph& g, const uint16_t* queries, uint64_t nq, uint3
 
 }  // namespace
 
-// Handle lookup and error reporting for entry points defined in other files
-// of this library (noalloc.cu).
+// Handle lookup, error reporting and per-call scratch for entry points defined
+// in other files of this library (noalloc.cu, paged_capi.cu).
 namespace jb {
+void capi_pool_alloc(void** p, size_t bytes, cudaStream_t st) { pool_alloc(p, bytes, st, "alloc scratch"); }
 std::shared_ptr<Graph> capi_lookup(int64_t h) { return lookup(h); }
 int capi_guarded(const std::function<void()>& f) { return guarded(f); }
 }  // namespace jb
