@@ -150,3 +150,26 @@ def call(name: str, *args) -> None:
         if rc == JB_ERR_IO:
             raise OSError(msg)
         raise JasperError(rc, msg)
+
+
+_paged = None
+
+
+def paged_module():
+    """lib/jasper_paged_torch.so, the paged cache's torch boundary, calling the
+    library that lib() loaded."""
+    global _paged
+    if _paged is None:
+        import importlib.util
+        path = Path(__file__).resolve().parent / "lib" / "jasper_paged_torch.so"
+        if not path.exists():
+            raise ImportError(f"{path} is missing: build it with `python -m jasper_b200.build`")
+        L = lib()
+        spec = importlib.util.spec_from_file_location("jasper_paged_torch", path)
+        m = importlib.util.module_from_spec(spec)
+        spec.loader.exec_module(m)
+        names = ["jb_last_error", *(n for n in SIGNATURES
+                                    if n.startswith(("jb_pages_", "jb_kv_", "jb_rotary", "jb_paged_")))]
+        m.init(JasperError, {n: C.cast(getattr(L, n), C.c_void_p).value for n in names})
+        _paged = m
+    return _paged

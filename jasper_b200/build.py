@@ -1,4 +1,5 @@
-"""Build recipe for libjasper_b200.so (sm_100a) and the tvm_ffi module.
+"""Build recipe for libjasper_b200.so (sm_100a), the tvm_ffi module and the
+paged cache's torch module.
 
 Compiles every CUDA source under ``jasper_b200/csrc`` with nvcc for
 ``-gencode arch=compute_100a,code=sm_100a`` into ``jasper_b200/lib``.  Objects
@@ -64,7 +65,33 @@ def build(verbose: bool = False) -> Path:
         if verbose:
             print("built", so)
     _build_tvm_module(so, verbose)
+    _build_paged_module(verbose)
     return so
+
+
+def _build_paged_module(verbose: bool) -> Path:
+    """lib/jasper_paged_torch.so: the paged cache's torch boundary (a CPython
+    module; it gets the C ABI's addresses from the loaded library)."""
+    import sysconfig
+
+    import torch
+    from torch.utils.cpp_extension import include_paths
+    src = CSRC / "paged_torch.cc"
+    out = LIB / "jasper_paged_torch.so"
+    if out.exists() and out.stat().st_mtime > max(src.stat().st_mtime, _headers_mtime()):
+        return out
+    torch_lib = Path(torch.__file__).resolve().parent / "lib"
+    cmd = ["g++", "-std=c++17", "-O2", "-fPIC", "-shared", "-fvisibility=hidden", "-o", str(out), str(src),
+           f"-I{sysconfig.get_paths()['include']}", *(f"-I{p}" for p in include_paths()),
+           "-I/usr/local/cuda/include", f"-D_GLIBCXX_USE_CXX11_ABI={int(torch.compiled_with_cxx11_abi())}",
+           f"-L{torch_lib}", "-ltorch_python", "-ltorch", "-ltorch_cpu", "-ltorch_cuda", "-lc10",
+           "-lc10_cuda", f"-Wl,-rpath,{torch_lib}"]
+    r = subprocess.run(cmd, capture_output=True, text=True)
+    if r.returncode != 0:
+        raise RuntimeError("paged torch module build failed:\n" + r.stderr)
+    if verbose:
+        print("built", out)
+    return out
 
 
 def _tvm_include() -> Path | None:

@@ -13,7 +13,8 @@ there.
   copying pages; appending new (rotated) keys and values; the attention of one
   new token of each row.
 
-The kernels are those of libjasper_b200.so (``jb_rotary``, ``jb_kv_append``,
+Tensors are checked and passed on by a small CPython module
+(csrc/paged_torch.cc); the kernels are those of libjasper_b200.so (``jb_rotary``, ``jb_kv_append``,
 ``jb_pages_*``, ``jb_paged_attention`` in include/jasper_b200.h).  Calls are
 asynchronous on torch's current stream of the cache's device and read nothing
 back: a row or page that does not fit sets a bit of the cache's status word,
@@ -38,32 +39,6 @@ _STATUS = {
     BAD_ROW: "a row is out of range, named twice, too long for the table or not empty",
     BAD_TOKEN: "a token's place or a page's number is out of range",
 }
-
-
-def _stream(device: torch.device) -> int:
-    return torch.cuda.current_stream(device).cuda_stream
-
-
-def _heads(t: torch.Tensor, name: str, heads: int | None, dim: int, dtype: torch.dtype,
-           device: torch.device) -> torch.Tensor:
-    """[tokens, heads, dim] with dim contiguous, on the device."""
-    if t.ndim != 3 or t.size(2) != dim or (heads is not None and t.size(1) != heads):
-        raise ValueError(f"{name} must be [n, {'heads' if heads is None else heads}, {dim}], "
-                         f"got {list(t.shape)}")
-    if t.dtype != dtype:
-        raise ValueError(f"{name} must be {dtype}, got {t.dtype}")
-    if t.device != device:
-        raise ValueError(f"{name} must be on {device}, got {t.device}")
-    return t if t.stride(2) == 1 or dim == 1 else t.contiguous()
-
-
-def _ints(t: torch.Tensor, name: str, n: int | None, device: torch.device) -> torch.Tensor:
-    if t.dtype != torch.int32 or t.device != device or t.ndim != 1:
-        raise ValueError(f"{name} must be a 1D int32 tensor on {device}, got {t.ndim}D {t.dtype} "
-                         f"on {t.device}")
-    if n is not None and t.size(0) != n:
-        raise ValueError(f"{name} must have {n} entries, got {t.size(0)}")
-    return t if t.stride(0) == 1 or t.size(0) <= 1 else t.contiguous()
 
 
 class Rotary:
@@ -122,6 +97,7 @@ class Rotary:
         self._freq = torch.tensor([t - 2 ** 64 if t >= 2 ** 63 else t for t in turns],
                                   dtype=torch.int64).to(device)
         self.device = self._freq.device
+        self._args = (self._freq, head_dim, rot_dim, self.scale, layout == "interleaved")
 
     def apply(self, x: torch.Tensor, positions: torch.Tensor,
               out: torch.Tensor | None = None) -> torch.Tensor:
@@ -131,48 +107,14 @@ class Rotary:
         ``out`` may be ``x``.  Differentiable in ``x`` unless ``out`` is given."""
         if out is None and x.requires_grad and torch.is_grad_enabled():
             return _Turn.apply(x, positions, self)
-        return self._turn(x, positions, out, False)
+        return _lib.paged_module().rotary(x, positions, out, False, *self._args)
 
     __call__ = apply
 
     def grad(self, dy: torch.Tensor, positions: torch.Tensor,
              out: torch.Tensor | None = None) -> torch.Tensor:
         """The gradient with respect to apply()'s ``x``, given its output's."""
-        return self._turn(dy, positions, out, True)
-
-    def _turn(self, x, positions, out, inverse):
-        if out is None:
-            out = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-        elif out.shape != x.shape or out.dtype != x.dtype or out.device != x.device:
-            raise ValueError("out must have x's shape, type and device")
-        if x.ndim == 4:
-            if out.stride(0) != out.size(1) * out.stride(1) and out.size(0) > 1:
-                raise ValueError("out's batch and tokens must be one run of tokens")
-            positions = positions.expand(x.shape[:2]).reshape(-1)
-            self._turn(x.flatten(0, 1), positions, out.flatten(0, 1), inverse)
-            return out
-        if x.dtype not in _DTYPES:
-            raise ValueError(f"Unsupported tensor dtype: {x.dtype}")
-        x = _heads(x, "x", None, self.head_dim, x.dtype, self.device)
-        if out.stride(2) != 1:
-            raise ValueError("out's heads must be contiguous")
-        n = x.size(0)
-        p64 = positions.dtype == torch.int64
-        if not p64 and positions.dtype != torch.int32:
-            raise ValueError(f"positions must be int32 or int64, got {positions.dtype}")
-        if positions.shape != (n,) or positions.device != self.device:
-            raise ValueError(f"positions must be [{n}] on {self.device}")
-        positions = positions.contiguous()
-        args = (x.data_ptr(), x.stride(0), x.stride(1), out.data_ptr(), out.stride(0), out.stride(1),
-                _DTYPES[x.dtype], n, x.size(1), self.head_dim, self.rot_dim, positions.data_ptr(), p64,
-                self._freq.data_ptr(), self.scale, self.layout == "interleaved", inverse,
-                _stream(self.device))
-        if torch.cuda.current_device() == self.device.index:
-            _lib.call("jb_rotary", *args)
-        else:
-            with torch.cuda.device(self.device):
-                _lib.call("jb_rotary", *args)
-        return out
+        return _lib.paged_module().rotary(dy, positions, out, True, *self._args)
 
 
 class _Turn(torch.autograd.Function):
@@ -180,11 +122,11 @@ class _Turn(torch.autograd.Function):
     def forward(ctx, x, positions, rotary):
         ctx.rotary = rotary
         ctx.save_for_backward(positions)
-        return rotary._turn(x, positions, None, False)
+        return _lib.paged_module().rotary(x, positions, None, False, *rotary._args)
 
     @staticmethod
     def backward(ctx, dy):
-        return ctx.rotary._turn(dy, ctx.saved_tensors[0], None, True), None, None
+        return ctx.rotary.grad(dy, ctx.saved_tensors[0]), None, None
 
 
 class PagedCache:
@@ -235,6 +177,7 @@ class PagedCache:
             status.data_ptr(), *k.stride()[:4], table.stride(0), *k.shape, *table.shape,
             _DTYPES[k.dtype], device.index)
         self._ref = C.addressof(self._c)
+        self._native = _lib.paged_module()
 
     @classmethod
     def allocate(cls, n_layers: int, n_pages: int, page_size: int, n_kv_heads: int, head_dim: int,
@@ -262,55 +205,32 @@ class PagedCache:
         its last one is full (the lowest free ones), and a length that counts
         them.  Rows are served in order; from the first that finds too few
         free pages on, rows that need pages stay as they were."""
-        rows = _ints(rows, "rows", None, self.device)
-        tokens = _ints(tokens, "tokens", rows.size(0), self.device)
-        _lib.call("jb_pages_extend", self._ref, rows.data_ptr(), tokens.data_ptr(), rows.size(0),
-                  _stream(self.device))
+        self._native.extend(self._ref, rows, tokens)
 
     def fork(self, parents: torch.Tensor, children: torch.Tensor) -> None:
         """Makes the empty rows ``children`` copies of ``parents``: whole pages
         are shared, a part-filled page is copied, so that each goes on alone."""
-        parents = _ints(parents, "parents", None, self.device)
-        children = _ints(children, "children", parents.size(0), self.device)
-        _lib.call("jb_pages_fork", self._ref, parents.data_ptr(), children.data_ptr(),
-                  parents.size(0), _stream(self.device))
+        self._native.fork(self._ref, parents, children)
 
     def free(self, rows: torch.Tensor) -> None:
         """Empties rows; pages that no row holds any more are free."""
-        rows = _ints(rows, "rows", None, self.device)
-        _lib.call("jb_pages_free", self._ref, rows.data_ptr(), rows.size(0), _stream(self.device))
+        self._native.free(self._ref, rows)
 
     def adopt(self, rows: torch.Tensor, pages: torch.Tensor, lengths: torch.Tensor | None = None) -> None:
         """Makes the empty rows ``rows`` further holders of ``pages`` (int32
         [len(rows), m]; -1: not there), whole or, with ``lengths``, the first
         lengths[i] tokens of them: a search's ids become rows to attend to."""
-        rows = _ints(rows, "rows", None, self.device)
-        if pages.dtype != torch.int32 or pages.ndim != 2 or pages.device != self.device:
-            raise ValueError(f"pages must be a 2D int32 tensor on {self.device}")
-        if pages.size(0) != rows.size(0):
-            raise ValueError(f"pages must have {rows.size(0)} rows, got {pages.size(0)}")
-        if pages.size(1) > 1 and pages.stride(1) != 1:
-            pages = pages.contiguous()
-        if lengths is not None:
-            lengths = _ints(lengths, "lengths", rows.size(0), self.device)
-        _lib.call("jb_pages_adopt", self._ref, rows.data_ptr(), pages.data_ptr(), pages.stride(0),
-                  pages.size(1), None if lengths is None else lengths.data_ptr(), rows.size(0),
-                  _stream(self.device))
+        self._native.adopt(self._ref, rows, pages, lengths)
 
     def compact(self) -> torch.Tensor:
         """Moves the live pages to the lowest numbers.  Returns int32 [pages]:
         each page's new number, -1 for one that was free."""
-        remap = torch.empty(self.n_pages, dtype=torch.int32, device=self.device)
-        _lib.call("jb_pages_compact", self._ref, remap.data_ptr(), _stream(self.device))
-        return remap
+        return self._native.compact(self._ref)
 
     def copy_pages(self, src: torch.Tensor, dst: torch.Tensor) -> None:
         """Copies keys and values of pages ``src`` to pages ``dst``, in every
         layer (no page twice in ``dst``, none in both)."""
-        src = _ints(src, "src", None, self.device)
-        dst = _ints(dst, "dst", src.size(0), self.device)
-        _lib.call("jb_pages_copy", self._ref, src.data_ptr(), dst.data_ptr(), src.size(0),
-                  _stream(self.device))
+        self._native.copy_pages(self._ref, src, dst)
 
     # ── tokens ─────────────────────────────────────────────────────────
     def append(self, layer: int, k: torch.Tensor, v: torch.Tensor, rows: torch.Tensor,
@@ -322,46 +242,8 @@ class PagedCache:
         the room).  With ``rotary``, keys are turned by ``positions`` (default:
         the index) on the way, and so is ``q`` [tokens, heads, head_dim], which
         is returned (in ``q_out`` if given, which may be ``q``)."""
-        dev, dim = self.device, self.head_dim
-        k = _heads(k, "k", self.n_kv_heads, dim, self.dtype, dev)
-        v = _heads(v, "v", self.n_kv_heads, dim, self.dtype, dev)
-        n = k.size(0)
-        if v.size(0) != n:
-            raise ValueError(f"v must have {n} tokens, got {v.size(0)}")
-        rows = _ints(rows, "rows", n, dev)
-        if index is not None:
-            index = _ints(index, "index", n, dev)
-        if q is None:
-            q_args = (None, 0, 0, None, 0, 0, 0)
-        else:
-            if rotary is None:
-                raise ValueError("q is only taken to be rotated: pass rotary")
-            q = _heads(q, "q", None, dim, self.dtype, dev)
-            if q.size(0) != n:
-                raise ValueError(f"q must have {n} tokens, got {q.size(0)}")
-            if q_out is None:
-                q_out = torch.empty(q.shape, dtype=q.dtype, device=dev)
-            elif q_out.shape != q.shape or q_out.dtype != q.dtype or q_out.device != dev or q_out.stride(2) != 1:
-                raise ValueError("q_out must have q's shape, type and device, and contiguous heads")
-            q_args = (q.data_ptr(), q.stride(0), q.stride(1), q_out.data_ptr(), q_out.stride(0),
-                      q_out.stride(1), q.size(1))
-        p64 = False
-        if positions is not None:
-            p64 = positions.dtype == torch.int64
-            if (not p64 and positions.dtype != torch.int32) or positions.shape != (n,) or positions.device != dev:
-                raise ValueError(f"positions must be int32 or int64 [{n}] on {dev}")
-            positions = positions.contiguous()
-        if rotary is None:
-            r_args = (None, 0, 1.0, 0)
-        elif rotary.head_dim != dim or rotary.device != dev:
-            raise ValueError(f"rotary must be for heads of {dim} on {dev}")
-        else:
-            r_args = (rotary._freq.data_ptr(), rotary.rot_dim, rotary.scale, rotary.layout == "interleaved")
-        _lib.call("jb_kv_append", self._ref, layer, n, *q_args, k.data_ptr(), k.stride(0), k.stride(1),
-                  v.data_ptr(), v.stride(0), v.stride(1), rows.data_ptr(),
-                  None if index is None else index.data_ptr(),
-                  None if positions is None else positions.data_ptr(), p64, *r_args, _stream(dev))
-        return q_out if q is not None else None
+        r = (None, 0, 0, 1.0, False) if rotary is None else rotary._args
+        return self._native.append(self._ref, layer, k, v, rows, index, q, positions, q_out, *r)
 
     def attend(self, layer: int, q: torch.Tensor, rows: torch.Tensor | None = None, *,
                scale: float | None = None, window: int = 0, mask: torch.Tensor | None = None,
@@ -374,40 +256,7 @@ class PagedCache:
         heads, head_dim], zeros where nothing is attended to; with
         ``return_lse`` also float32 [n, heads], log sum exp of the scores
         (-inf there)."""
-        dev = self.device
-        q = _heads(q, "q", None, self.head_dim, self.dtype, dev)
-        n, heads, dim = q.shape
-        if heads % self.n_kv_heads:
-            raise ValueError(f"q's heads ({heads}) must be a multiple of the cache's ({self.n_kv_heads})")
-        if q.stride(0) % 8 or q.stride(1) % 8 or q.data_ptr() % 16:
-            q = q.contiguous()
-            if q.data_ptr() % 16:
-                q = q.clone()
-        if rows is not None:
-            rows = _ints(rows, "rows", n, dev)
-        elif n > self.n_rows:
-            raise ValueError(f"q has {n} rows, the cache {self.n_rows}")
-        if window < 0:
-            raise ValueError(f"window must not be negative, got {window}")
-        if mask is None:
-            m_args = (None, 0, 0)
-        else:
-            if mask.dtype != torch.bool or mask.ndim != 2 or mask.size(0) != n or mask.device != dev:
-                raise ValueError(f"mask must be bool [{n}, width] on {dev}")
-            if mask.size(1) > 1 and mask.stride(1) != 1:
-                mask = mask.contiguous()
-            m_args = (mask.data_ptr(), mask.stride(0), mask.size(1))
-        if out is None:
-            out = torch.empty((n, heads, dim), dtype=q.dtype, device=dev)
-        elif out.shape != q.shape or out.dtype != q.dtype or out.device != dev or out.stride(2) != 1:
-            raise ValueError("out must have q's shape, type and device, and contiguous heads")
-        lse = torch.empty((n, heads), dtype=torch.float32, device=dev) if return_lse else None
-        _lib.call("jb_paged_attention", self._ref, layer, q.data_ptr(), q.stride(0), q.stride(1),
-                  out.data_ptr(), out.stride(0), out.stride(1), n, heads,
-                  None if rows is None else rows.data_ptr(), *m_args, window,
-                  dim ** -0.5 if scale is None else scale, None if lse is None else lse.data_ptr(),
-                  _stream(dev))
-        return (out, lse) if return_lse else out
+        return self._native.attend(self._ref, layer, q, rows, scale, window, mask, return_lse, out)
 
     def check(self) -> None:
         """Waits for the cache's stream, and raises what the calls since the
