@@ -1,12 +1,35 @@
 // attend.cu -- attention of one new token of each row over the paged cache.
 //
 // out = sum_t p_t v_t, p = softmax(scale * q . k_t) over the tokens attended
-// to, in one pass with the running maximum m and sum l of the softmax: a
-// score above m rescales what was gathered by exp(m_old - m_new).
+// to, in one pass over keys and values with the running reference r and sum l
+// of the softmax: weights are 2^(s - r), and a score far above r moves it and
+// rescales what was gathered.
 //
-// One warp per (row, query head): each lane holds head_dim / 32 of the
-// query's and the output's elements.
+// What bounds it: every key and value is read once and used for a group of at
+// most 16 query heads, 2 to 32 flops a byte, so HBM.  The rest is keeping
+// enough bytes in flight and every SM equally long at work:
+//
+//  * A warp is a worker of its own.  All rows' tiles of TK tokens, one row's
+//    head after the other, form one line, and worker w of W takes the w-th of
+//    W equal parts, whatever the rows' lengths.  A row's head that lies in one
+//    part is finished there; one that spans several leaves a part result in
+//    each, and a second kernel joins them in order (no atomics: equal inputs
+//    give equal bits).
+//  * The worker's tiles stream through its own ring of STAGES tiles in shared
+//    memory by 16-byte cp.async, over the borders of rows, with no block-wide
+//    barrier.  Tokens that are not attended to are not read: their rows are
+//    filled with zeros, whatever the cache holds there.
+//  * Products run on mma.sync m16n8k16 with tokens (then head elements) as the
+//    16 rows and query heads as the 8 columns, S^T = K Q^T and O^T = V^T P^T,
+//    so a group of 8 heads wastes nothing; movmatrix turns the weights from
+//    accumulator to operand.  tcgen05 has nothing to give here: its smallest
+//    tile is 64 rows or columns of queries wide, and the tensor pipe is far
+//    from busy.
+//  * A weight enters the second product as the sum of two 16-bit values (its
+//    rounding, and the rounding of what that left), so nothing is lost
+//    against float32 weights; l sums the float32 weights.
 #include <cmath>
+#include <mutex>
 #include <stdexcept>
 #include <string>
 #include "paged.cuh"
@@ -14,90 +37,756 @@
 namespace jb {
 namespace {
 
-constexpr int kMaxPerLane = 8;  // head_dim up to 256
+constexpr uint32_t kFullMask = 0xFFFFFFFFu;
+constexpr int kMaxListed = 1024;  // queries whose lengths a block keeps in shared memory
+// A weight is 2^(s - r): r is set 6 below the largest score and stays until a
+// score is 15 above it, so weights reach 2^15, inside float16, and the largest
+// is at least 2^6: float16 weights keep 24 + 6 bits below the largest.
+constexpr float kRefBelow = 6.0f, kRefRoom = 15.0f;
 
 template <typename T>
-__device__ __forceinline__ float to_float(T v);
+struct Mma;
 template <>
-__device__ __forceinline__ float to_float<__half>(__half v) { return __half2float(v); }
+struct Mma<__half> {
+  static __device__ __forceinline__ void mma(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    asm volatile(
+        "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+  }
+  // (a, b) to 16 bits, and what that left, to 16 bits again
+  static __device__ __forceinline__ void split(float a, float b, uint32_t& hi, uint32_t& lo) {
+    const __half2 h = __floats2half2_rn(a, b);
+    const float2 f = __half22float2(h);
+    const __half2 l = __floats2half2_rn(a - f.x, b - f.y);
+    hi = *reinterpret_cast<const uint32_t*>(&h);
+    lo = *reinterpret_cast<const uint32_t*>(&l);
+  }
+  static __device__ __forceinline__ __half from(float v) { return __float2half_rn(v); }
+};
 template <>
-__device__ __forceinline__ float to_float<__nv_bfloat16>(__nv_bfloat16 v) { return __bfloat162float(v); }
-template <typename T>
-__device__ __forceinline__ T from_float(float v);
-template <>
-__device__ __forceinline__ __half from_float<__half>(float v) { return __float2half_rn(v); }
-template <>
-__device__ __forceinline__ __nv_bfloat16 from_float<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
+struct Mma<__nv_bfloat16> {
+  static __device__ __forceinline__ void mma(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    asm volatile(
+        "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+  }
+  static __device__ __forceinline__ void split(float a, float b, uint32_t& hi, uint32_t& lo) {
+    const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
+    const float2 f = __bfloat1622float2(h);
+    const __nv_bfloat162 l = __floats2bfloat162_rn(a - f.x, b - f.y);
+    hi = *reinterpret_cast<const uint32_t*>(&h);
+    lo = *reinterpret_cast<const uint32_t*>(&l);
+  }
+  static __device__ __forceinline__ __nv_bfloat16 from(float v) { return __float2bfloat16_rn(v); }
+};
 
-template <typename T>
-__global__ void __launch_bounds__(32) attend_warp_kernel(const AttendArgs a) {
-  const jb_page_cache& c = a.c;
-  const uint32_t i = blockIdx.x / a.n_q_heads, hq = blockIdx.x % a.n_q_heads;
-  const uint32_t h = hq / (a.n_q_heads / c.n_kv_heads);
-  const int lane = threadIdx.x;
-  const int32_t row = a.rows ? a.rows[i] : int32_t(i);
+__device__ __forceinline__ uint32_t smem_addr(const void* p) {
+  return static_cast<uint32_t>(__cvta_generic_to_shared(p));
+}
+__device__ __forceinline__ void ldmatrix(uint32_t (&r)[4], uint32_t addr) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
+}
+__device__ __forceinline__ void ldmatrix_trans(uint32_t (&r)[4], uint32_t addr) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
+}
+__device__ __forceinline__ uint32_t transposed(uint32_t v) {
+  uint32_t r;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
+  return r;
+}
+// 16 bytes to shared memory, or 16 zeros
+__device__ __forceinline__ void copy16(uint32_t dst, const void* src, bool real) {
+  const int n = real ? 16 : 0;
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(n) : "memory");
+}
+__device__ __forceinline__ void copies_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void copies_wait() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+__device__ __forceinline__ float exp2_fast(float x) {
+  float r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
+}
+
+// Where the part results of a call lie: worker w has slot 2w for a row's head
+// that began before its part, slot 2w + 1 for one that goes on behind it.
+struct Parts {
+  float* o;        // [2 W][columns][DP]
+  float2* rl;      // [2 W][columns]: reference and sum
+  int4* spans;     // the rows' heads that lie in several parts: query, head
+                   // tile, parts (0: none), first worker.  One entry for
+                   // each row's head, or, if fewer, for each worker (in
+                   // whose part at most one begins that goes on behind it)
+  int64_t* prefix; // [n + 1] tiles before each query; null: blocks sum them
+};
+
+struct AttendParams {
+  AttendArgs a;
+  Parts parts;
+  uint32_t group, head_tiles;  // query heads of a key-value head, and tiles of 8 NT of them
+  uint32_t workers;
+  bool by_worker;              // what parts.spans goes by
+};
+
+// The tiles of TK tokens that query i reads.
+struct Tiles {
+  int32_t row, len, first, begin, end;
+};
+template <int TK>
+__device__ __forceinline__ Tiles tiles_of(const AttendArgs& a, uint32_t i) {
+  Tiles t;
+  t.row = a.rows ? a.rows[i] : int32_t(i);
   int64_t len = 0;
-  if (row >= 0 && uint32_t(row) < c.n_rows)
-    len = min(int64_t(max(c.lengths[row], 0)), int64_t(c.max_pages) * c.page_size);
-  const int64_t first = a.window && len > int64_t(a.window) ? len - a.window : 0;
-  const T* q = static_cast<const T*>(a.q.p) + i * a.q.token_stride + hq * a.q.head_stride;
-  const T* k = static_cast<const T*>(c.k) + int64_t(a.layer) * c.layer_stride + h * c.head_stride;
-  const T* v = static_cast<const T*>(c.v) + int64_t(a.layer) * c.layer_stride + h * c.head_stride;
-  float qf[kMaxPerLane], o[kMaxPerLane];
+  if (t.row >= 0 && uint32_t(t.row) < a.c.n_rows)
+    len = min(int64_t(max(a.c.lengths[t.row], 0)), int64_t(a.c.max_pages) * a.c.page_size);
+  t.len = int32_t(len);
+  t.first = a.window && len > int64_t(a.window) ? int32_t(len - a.window) : 0;
+  t.begin = t.first / TK;
+  t.end = int32_t((len + TK - 1) / TK);
+  return t;
+}
+
+// Inclusive sum over the block's threads (256 at most) of one value each.
+template <int THREADS>
+__device__ __forceinline__ int64_t block_sum_scan(int64_t v, int64_t* total) {
+  __shared__ int64_t sums[THREADS / 32];
+  const int lane = threadIdx.x & 31, wid = threadIdx.x >> 5;
 #pragma unroll
-  for (int j = 0; j < kMaxPerLane; j++) {
-    const uint32_t d = lane + 32 * j;
-    qf[j] = d < c.head_dim ? to_float(q[d]) * a.scale : 0.0f;
-    o[j] = 0.0f;
+  for (int d = 1; d < 32; d <<= 1) {
+    const int64_t y = __shfl_up_sync(kFullMask, v, d);
+    if (lane >= d) v += y;
   }
-  float m = -INFINITY, l = 0.0f;
-  for (int64_t t = first; t < len; t++) {
-    if (a.mask && t < a.mask_width && !a.mask[i * a.mask_stride + t]) continue;
-    const int32_t page = c.table[row * c.table_stride + t / c.page_size];
-    if (page < 0 || uint32_t(page) >= c.n_pages) continue;
-    const int64_t off = page * c.page_stride + (t % c.page_size) * c.token_stride;
-    float s = 0.0f;
+  if (lane == 31) sums[wid] = v;
+  __syncthreads();
+  int64_t before = 0, all = 0;
 #pragma unroll
-    for (int j = 0; j < kMaxPerLane; j++) {
-      const uint32_t d = lane + 32 * j;
-      if (d < c.head_dim) s += qf[j] * to_float(k[off + d]);
+  for (int i = 0; i < THREADS / 32; i++) {
+    if (i < wid) before += sums[i];
+    all += sums[i];
+  }
+  __syncthreads();
+  *total = all;
+  return v + before;
+}
+
+// The tiles before each query, for more queries than a block keeps itself.
+template <int TK>
+__global__ void __launch_bounds__(1024) prefix_kernel(const AttendArgs a, int64_t* prefix) {
+  int64_t done = 0;
+  for (uint64_t base = 0; base < a.n; base += 1024) {
+    const uint64_t i = base + threadIdx.x;
+    int64_t v = 0;
+    if (i < a.n) {
+      const Tiles t = tiles_of<TK>(a, uint32_t(i));
+      v = max(t.end - t.begin, 0);
+    }
+    int64_t total;
+    const int64_t upto = done + block_sum_scan<1024>(v, &total);
+    if (i < a.n) prefix[i + 1] = upto;
+    done += total;
+  }
+  if (threadIdx.x == 0) prefix[0] = 0;
+}
+
+// Bytes from a row of a tile in shared memory to the next.  Eight consecutive
+// rows at the same column must fall into different banks for ldmatrix: where
+// rows are whole multiples of 128 bytes the 16-byte chunks are permuted by the
+// row's last three bits, else an odd number of chunks lies between rows.
+template <int DP>
+struct TileLayout {
+  static constexpr bool kPermuted = (DP * 2) % 128 == 0;
+  static constexpr int kRowBytes = kPermuted ? DP * 2 : DP * 2 + 16;
+  static __device__ __forceinline__ uint32_t at(int row, int chunk) {
+    return row * kRowBytes + (kPermuted ? (chunk ^ (row & 7)) : chunk) * 16;
+  }
+};
+
+// A place in the line of tiles: a query's head tile, and its tile.
+struct Cursor {
+  Tiles t;
+  uint32_t i, vh;
+  int32_t tile;
+};
+
+template <typename T, int DP, int NT, int TK, int WARPS, int STAGES>
+struct Attend {
+  using L = TileLayout<DP>;
+  static constexpr int kThreads = WARPS * 32;
+  static constexpr int kColumns = 8 * NT;
+  static constexpr int kTileBytes = TK * L::kRowBytes;   // keys, then as much values
+  static constexpr int kStageBytes = 2 * kTileBytes;
+  static constexpr int kRingBytes = WARPS * STAGES * kStageBytes;
+  static constexpr int kSmem = kRingBytes + WARPS * STAGES * 4 + kMaxListed * 8 + (kMaxListed + 1) * 8 + 8;
+  static constexpr int KS = DP / 16;                     // k steps of Q K, head tiles of 16 of P V
+  static constexpr int MT = TK / 16;
+  static constexpr int kChunkLanes = DP <= 64 ? 8 : DP <= 128 ? 16 : 32;  // lanes a row of 16-byte chunks takes
+  static constexpr int kRowsPerCopy = 32 / kChunkLanes;
+
+  struct Lists {
+    int32_t *row, *len;
+    int64_t* prefix;
+  };
+
+  const AttendParams& p;
+  const Lists& lists;
+  int lane;
+
+  __device__ __forceinline__ Tiles load_tiles(uint32_t i) const {
+    if (p.parts.prefix) return tiles_of<TK>(p.a, i);
+    Tiles t;
+    t.row = lists.row[i];
+    t.len = lists.len[i];
+    t.first = p.a.window && t.len > int64_t(p.a.window) ? int32_t(t.len - p.a.window) : 0;
+    t.begin = t.first / TK;
+    t.end = int32_t((int64_t(t.len) + TK - 1) / TK);
+    return t;
+  }
+  __device__ __forceinline__ uint32_t head_rows() const { return p.a.c.n_kv_heads * p.head_tiles; }
+
+  __device__ __forceinline__ void next(Cursor& c) const {
+    if (++c.tile < c.t.end) return;
+    c.tile = c.t.begin;
+    if (++c.vh < head_rows()) return;
+    c.vh = 0;
+    do {
+      if (++c.i >= p.a.n) return;
+      c.t = load_tiles(c.i);
+    } while (c.t.end <= c.t.begin);
+    c.tile = c.t.begin;
+  }
+
+  // Page of the lane's token in a tile; -1 where it is not attended to.
+  __device__ __forceinline__ int32_t page_of(const Cursor& c, uint32_t& slot) const {
+    const int64_t t = int64_t(c.tile) * TK + lane;
+    int32_t page = -1;
+    slot = 0;
+    if (lane < TK && t >= c.t.first && t < c.t.len) {
+      const uint32_t pg = uint32_t(t) / p.a.c.page_size;
+      slot = uint32_t(t) - pg * p.a.c.page_size;
+      const bool kept = !p.a.mask || t >= p.a.mask_width || p.a.mask[int64_t(c.i) * p.a.mask_stride + t];
+      if (kept) page = p.a.c.table[c.t.row * p.a.c.table_stride + pg];
+      if (page >= 0 && uint32_t(page) >= p.a.c.n_pages) page = -1;
+    }
+    return page;
+  }
+
+  __device__ __forceinline__ void load_tile(uint32_t stage, uint32_t* valid, const Cursor& c, int32_t page,
+                                            uint32_t slot) const {
+    const jb_page_cache& k = p.a.c;
+    const uint32_t mask = __ballot_sync(kFullMask, page >= 0);
+    if (lane == 0) *valid = mask;
+    if (mask) {
+      const int64_t base = int64_t(p.a.layer) * k.layer_stride + (c.vh / p.head_tiles) * k.head_stride;
+      const int64_t mine = base + (page >= 0 ? page * k.page_stride + slot * k.token_stride : 0);
+      const int chunk = lane % kChunkLanes;
+      const bool inside = chunk < int(k.head_dim / 8);
+#pragma unroll
+      for (int it = 0; it < TK / kRowsPerCopy; it++) {
+        const int row = it * kRowsPerCopy + lane / kChunkLanes;
+        const int64_t off = __shfl_sync(kFullMask, mine, row) + chunk * 8;
+        if (inside) {
+          const bool real = (mask >> row) & 1;
+          const uint32_t dst = stage + L::at(row, chunk);
+          copy16(dst, static_cast<const T*>(k.k) + off, real);
+          copy16(dst + kTileBytes, static_cast<const T*>(k.v) + off, real);
+        }
+      }
+    }
+  }
+
+  struct State {
+    float o[NT][KS][4];
+    float ref[NT][2], sum[NT][2];
+    uint32_t q[NT][KS][2];
+  };
+
+  __device__ __forceinline__ uint32_t head_of(uint32_t vh, int column) const {
+    return (vh / p.head_tiles) * p.group + (vh % p.head_tiles) * kColumns + column;
+  }
+  __device__ __forceinline__ bool head_real(uint32_t vh, int column) const {
+    return (vh % p.head_tiles) * kColumns + column < p.group;
+  }
+
+  __device__ __forceinline__ void begin(State& s, uint32_t i, uint32_t vh) const {
+#pragma unroll
+    for (int n = 0; n < NT; n++) {
+      const int column = 8 * n + lane / 4;
+      const T* q = static_cast<const T*>(p.a.q.p) + int64_t(i) * p.a.q.token_stride +
+                   int64_t(head_of(vh, column)) * p.a.q.head_stride;
+      const bool real = head_real(vh, column);
+#pragma unroll
+      for (int k = 0; k < KS; k++)
+#pragma unroll
+        for (int j = 0; j < 2; j++) {
+          const uint32_t d = 16 * k + 8 * j + 2 * (lane % 4);
+          s.q[n][k][j] = real && d < p.a.c.head_dim ? *reinterpret_cast<const uint32_t*>(q + d) : 0u;
+        }
+#pragma unroll
+      for (int k = 0; k < KS; k++)
+#pragma unroll
+        for (int j = 0; j < 4; j++) s.o[n][k][j] = 0.0f;
+      s.ref[n][0] = s.ref[n][1] = -INFINITY;
+      s.sum[n][0] = s.sum[n][1] = 0.0f;
+    }
+  }
+
+  __device__ __forceinline__ void tile(State& s, uint32_t stage, uint32_t mask) const {
+    // S^T: rows are tokens, columns are query heads
+    float w[NT][MT][4];
+#pragma unroll
+    for (int n = 0; n < NT; n++)
+#pragma unroll
+      for (int m = 0; m < MT; m++) w[n][m][0] = w[n][m][1] = w[n][m][2] = w[n][m][3] = 0.0f;
+#pragma unroll
+    for (int m = 0; m < MT; m++) {
+#pragma unroll
+      for (int k = 0; k < KS; k++) {
+        uint32_t a[4];
+        ldmatrix(a, stage + L::at(16 * m + (lane & 15), 2 * k + (lane >> 4)));
+#pragma unroll
+        for (int n = 0; n < NT; n++) Mma<T>::mma(w[n][m], a, s.q[n][k][0], s.q[n][k][1]);
+      }
+    }
+    const float scale = p.a.scale * 1.4426950408889634f;  // log2(e)
+    bool far = false;
+#pragma unroll
+    for (int n = 0; n < NT; n++)
+#pragma unroll
+      for (int m = 0; m < MT; m++)
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+          const int row = 16 * m + lane / 4 + 8 * (j / 2);
+          w[n][m][j] = (mask >> row) & 1 ? w[n][m][j] * scale : -INFINITY;
+          far |= w[n][m][j] > s.ref[n][j & 1] + kRefRoom;
+        }
+    if (__any_sync(kFullMask, far)) {
+#pragma unroll
+      for (int n = 0; n < NT; n++)
+#pragma unroll
+        for (int j = 0; j < 2; j++) {
+          float top = -INFINITY;
+#pragma unroll
+          for (int m = 0; m < MT; m++) top = fmaxf(top, fmaxf(w[n][m][j], w[n][m][j + 2]));
+#pragma unroll
+          for (int d = 4; d < 32; d <<= 1) top = fmaxf(top, __shfl_xor_sync(kFullMask, top, d));
+          const float ref = fmaxf(s.ref[n][j], top - kRefBelow);
+          const float keep = s.ref[n][j] == -INFINITY ? 0.0f : exp2_fast(s.ref[n][j] - ref);
+          s.ref[n][j] = ref;
+          s.sum[n][j] *= keep;
+#pragma unroll
+          for (int k = 0; k < KS; k++) {
+            s.o[n][k][j] *= keep;
+            s.o[n][k][j + 2] *= keep;
+          }
+        }
+    }
+    // O^T += V^T P^T: rows are head elements
+    uint32_t hi[NT][MT][2], lo[NT][MT][2];
+#pragma unroll
+    for (int n = 0; n < NT; n++) {
+      const float r0 = s.ref[n][0] == -INFINITY ? 0.0f : s.ref[n][0];
+      const float r1 = s.ref[n][1] == -INFINITY ? 0.0f : s.ref[n][1];
+#pragma unroll
+      for (int m = 0; m < MT; m++) {
+        const float a = exp2_fast(w[n][m][0] - r0), b = exp2_fast(w[n][m][1] - r1);
+        const float c = exp2_fast(w[n][m][2] - r0), d = exp2_fast(w[n][m][3] - r1);
+        s.sum[n][0] += a + c;
+        s.sum[n][1] += b + d;
+        Mma<T>::split(a, b, hi[n][m][0], lo[n][m][0]);
+        Mma<T>::split(c, d, hi[n][m][1], lo[n][m][1]);
+#pragma unroll
+        for (int j = 0; j < 2; j++) {
+          hi[n][m][j] = transposed(hi[n][m][j]);
+          lo[n][m][j] = transposed(lo[n][m][j]);
+        }
+      }
     }
 #pragma unroll
-    for (int w = 16; w; w >>= 1) s += __shfl_xor_sync(0xFFFFFFFFu, s, w);
-    const float mn = fmaxf(m, s);
-    const float keep = m == -INFINITY ? 0.0f : expf(m - mn);
-    const float p = mn == -INFINITY ? 0.0f : expf(s - mn);
-    m = mn;
-    l = l * keep + p;
+    for (int m = 0; m < MT; m++)
 #pragma unroll
-    for (int j = 0; j < kMaxPerLane; j++) {
-      const uint32_t d = lane + 32 * j;
-      if (d < c.head_dim) o[j] = o[j] * keep + p * to_float(v[off + d]);
-    }
+      for (int k = 0; k < KS; k++) {
+        uint32_t a[4];
+        ldmatrix_trans(a, stage + kTileBytes + L::at(16 * m + (lane & 7) + ((lane >> 4) << 3), 2 * k + ((lane >> 3) & 1)));
+#pragma unroll
+        for (int n = 0; n < NT; n++) {
+          Mma<T>::mma(s.o[n][k], a, hi[n][m][0], hi[n][m][1]);
+          Mma<T>::mma(s.o[n][k], a, lo[n][m][0], lo[n][m][1]);
+        }
+      }
   }
-  T* out = static_cast<T*>(a.out.p) + i * a.out.token_stride + hq * a.out.head_stride;
+
+  // The piece's end: the result, or a part of it (slot >= 0).
+  __device__ __forceinline__ void finish(State& s, uint32_t i, uint32_t vh, int64_t slot) const {
+#pragma unroll
+    for (int n = 0; n < NT; n++)
+#pragma unroll
+      for (int j = 0; j < 2; j++) {
+        float l = s.sum[n][j];
+#pragma unroll
+        for (int d = 4; d < 32; d <<= 1) l += __shfl_xor_sync(kFullMask, l, d);
+        const int column = 8 * n + 2 * (lane % 4) + j;
+        if (!head_real(vh, column)) continue;
+        const uint32_t h = head_of(vh, column);
+        if (slot >= 0) {
+          float* o = p.parts.o + (slot * kColumns + column) * DP;
+#pragma unroll
+          for (int k = 0; k < KS; k++) {
+            o[16 * k + lane / 4] = s.o[n][k][j];
+            o[16 * k + lane / 4 + 8] = s.o[n][k][j + 2];
+          }
+          if (lane < 4) p.parts.rl[slot * kColumns + column] = make_float2(s.ref[n][j], l);
+        } else {
+          T* out = static_cast<T*>(p.a.out.p) + int64_t(i) * p.a.out.token_stride + int64_t(h) * p.a.out.head_stride;
+          const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+#pragma unroll
+          for (int k = 0; k < KS; k++) {
+            const uint32_t d = 16 * k + lane / 4;
+            if (d < p.a.c.head_dim) out[d] = Mma<T>::from(s.o[n][k][j] * inv);
+            if (d + 8 < p.a.c.head_dim) out[d + 8] = Mma<T>::from(s.o[n][k][j + 2] * inv);
+          }
+          if (p.a.lse && lane < 4)
+            p.a.lse[int64_t(i) * p.a.n_q_heads + h] =
+                l == 0.0f ? -INFINITY : (s.ref[n][j] + log2f(l)) * 0.6931471805599453f;
+        }
+      }
+  }
+
+  // The last query whose tiles begin at or before `tile` (which is below the total).
+  __device__ __forceinline__ uint32_t query_at(int64_t tile) const {
+    const int64_t* pre = p.parts.prefix ? p.parts.prefix : lists.prefix;
+    uint32_t low = 0, high = p.a.n;  // pre[low] <= tile < pre[high]
+    while (high - low > 1) {         // 32 probes at a time
+      const uint32_t step = (high - low + 31) / 32;
+      const uint32_t probe = low + step * lane;
+      const bool under = probe < high && pre[probe] <= tile;
+      const int last = 31 - __clz(__ballot_sync(kFullMask, under));
+      low += step * last;
+      high = min(high, low + step);
+    }
+    return low;
+  }
+
+  __device__ __forceinline__ void work(uint32_t worker, unsigned char* ring, uint32_t* valid, int64_t total) const {
+    const int64_t each = total / p.workers, more = total % p.workers;
+    const int64_t w0 = int64_t(worker) * each + min(int64_t(worker), more);
+    int64_t left = each + (int64_t(worker) < more);
+    if (p.by_worker && lane == 0) p.parts.spans[worker] = make_int4(0, 0, 0, 0);
+    if (left == 0) return;
+    const uint32_t heads = head_rows();
+    Cursor c;
+    c.i = query_at(w0 / heads);
+    c.t = load_tiles(c.i);
+    const int64_t* pre = p.parts.prefix ? p.parts.prefix : lists.prefix;
+    const int64_t into = w0 - pre[c.i] * heads;
+    const int32_t count = c.t.end - c.t.begin;
+    c.vh = uint32_t(into / count);
+    c.tile = c.t.begin + int32_t(into % count);
+
+    Cursor ahead = c;       // the next tile to load
+    int64_t to_load = left;
+    uint32_t slot = 0;
+    int32_t page = page_of(ahead, slot);
+    const uint32_t stage0 = smem_addr(ring);
+    int load_stage = 0;
+    // loads the tile at `ahead`, and looks up the next one's pages
+    auto load_next = [&] {
+      if (to_load > 0) {
+        load_tile(stage0 + load_stage * kStageBytes, valid + load_stage, ahead, page, slot);
+        if (--to_load > 0) {
+          next(ahead);
+          page = page_of(ahead, slot);
+        }
+      }
+      copies_commit();
+      load_stage = load_stage + 1 == STAGES ? 0 : load_stage + 1;
+    };
+#pragma unroll
+    for (int s = 0; s < STAGES - 1; s++) load_next();
+
+    State s;
+    begin(s, c.i, c.vh);
+    bool whole = c.tile == c.t.begin;
+    int stage = 0;
+    for (;;) {
+      copies_wait<STAGES - 2>();
+      __syncwarp();
+      load_next();
+      const uint32_t mask = valid[stage];
+      if (mask) tile(s, stage0 + stage * kStageBytes, mask);
+      __syncwarp();
+      stage = stage + 1 == STAGES ? 0 : stage + 1;
+      left--;
+      const bool ends = c.tile + 1 == c.t.end;
+      if (ends || left == 0) {
+        const int64_t slot_of = ends ? (whole ? -1 : 2 * int64_t(worker)) : whole ? 2 * int64_t(worker) + 1 : 2 * int64_t(worker);
+        finish(s, c.i, c.vh, slot_of);
+        if (whole && lane == 0 && (!ends || !p.by_worker)) {
+          int parts = 0;
+          if (!ends) {  // the row's head goes on: in how many parts, this one included
+            const int64_t last = pre[c.i] * heads + (int64_t(c.vh) + 1) * (c.t.end - c.t.begin) - 1;
+            const int64_t border = more * (each + 1);
+            const int64_t last_worker = last < border ? last / (each + 1) : more + (last - border) / each;
+            parts = int(last_worker - worker + 1);
+          }
+          p.parts.spans[p.by_worker ? worker : c.i * heads + c.vh] =
+              make_int4(int(c.i), int(c.vh), parts, int(worker));
+        }
+        if (left == 0) break;
+        next(c);
+        begin(s, c.i, c.vh);
+        whole = true;
+      } else {
+        c.tile++;
+      }
+    }
+    copies_wait<0>();
+  }
+};
+
+template <typename T, int DP, int NT, int TK, int WARPS, int STAGES>
+__global__ void __launch_bounds__(WARPS * 32) attend_kernel(const __grid_constant__ AttendParams p) {
+  using A = Attend<T, DP, NT, TK, WARPS, STAGES>;
+  extern __shared__ __align__(128) unsigned char smem[];
+  uint32_t* valid = reinterpret_cast<uint32_t*>(smem + A::kRingBytes);
+  int64_t* prefix = reinterpret_cast<int64_t*>(smem + ((A::kRingBytes + WARPS * STAGES * 4 + 7) & ~7));
+  int32_t* row = reinterpret_cast<int32_t*>(prefix + kMaxListed + 1);
+  int32_t* len = row + kMaxListed;
+  typename A::Lists lists{row, len, prefix};
+  const int wid = threadIdx.x >> 5;
+  A self{p, lists, int(threadIdx.x & 31)};
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  if (p.a.c.head_dim < DP)  // columns that no copy writes
+    for (int i = threadIdx.x; i < A::kRingBytes / 16; i += A::kThreads)
+      reinterpret_cast<uint4*>(smem)[i] = make_uint4(0, 0, 0, 0);
+  int64_t total = 0;
+  if (p.parts.prefix) {
+    total = p.parts.prefix[p.a.n];
+  } else {
+    for (uint32_t base = 0; base < p.a.n; base += A::kThreads) {
+      const uint32_t i = base + threadIdx.x;
+      int64_t v = 0;
+      if (i < p.a.n) {
+        const Tiles t = tiles_of<TK>(p.a, i);
+        row[i] = t.row;
+        len[i] = t.len;
+        v = max(t.end - t.begin, 0);
+      }
+      int64_t sum;
+      const int64_t upto = total + block_sum_scan<A::kThreads>(v, &sum);
+      if (i < p.a.n) prefix[i + 1] = upto;
+      total += sum;
+    }
+    if (threadIdx.x == 0) prefix[0] = 0;
+  }
+  __syncthreads();
+  // queries with nothing to attend to
+  const int64_t* pre = p.parts.prefix ? p.parts.prefix : prefix;
+  for (uint32_t i = blockIdx.x; i < p.a.n; i += gridDim.x) {
+    if (pre[i + 1] != pre[i]) continue;
+    for (uint32_t j = threadIdx.x; j < p.a.n_q_heads * p.a.c.head_dim; j += A::kThreads)
+      static_cast<T*>(p.a.out.p)[int64_t(i) * p.a.out.token_stride +
+                                 int64_t(j / p.a.c.head_dim) * p.a.out.head_stride + j % p.a.c.head_dim] =
+          Mma<T>::from(0.0f);
+    if (p.a.lse)
+      for (uint32_t h = threadIdx.x; h < p.a.n_q_heads; h += A::kThreads)
+        p.a.lse[int64_t(i) * p.a.n_q_heads + h] = -INFINITY;
+    if (!p.by_worker)
+      for (uint32_t h = threadIdx.x; h < self.head_rows(); h += A::kThreads)
+        p.parts.spans[i * self.head_rows() + h] = make_int4(0, 0, 0, 0);
+  }
+  // neighbouring parts on different SMs, so that few tiles are spread over all
+  self.work(wid * gridDim.x + blockIdx.x, smem + wid * STAGES * A::kStageBytes, valid + wid * STAGES,
+            total * self.head_rows());
+}
+
+// Joins the parts of one row's head (span blockIdx.x), for one query head
+// (blockIdx.y): out = sum_i o_i 2^(r_i - r) / sum_i l_i 2^(r_i - r),
+// r the largest reference.  Eight warps take every eighth part each.
+template <typename T, int DP, int NT>
+__global__ void __launch_bounds__(256) join_kernel(const __grid_constant__ AttendParams p) {
+  constexpr int kColumns = 8 * NT;
+  __shared__ float share[8][DP];
+  __shared__ float reach[8], sums[8];
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  const int4 span = p.parts.spans[blockIdx.x];
+  const int column = blockIdx.y;
+  const uint32_t vh = uint32_t(span.y);
+  if (span.z == 0 || (vh % p.head_tiles) * kColumns + column >= p.group) return;
+  const int lane = threadIdx.x & 31, wid = threadIdx.x >> 5;
+  // part 0 is the first worker's last piece, part j > 0 the next workers' first
+  auto slot = [&](int j) { return (2 * (int64_t(span.w) + j) + (j == 0)) * kColumns + column; };
+  float top = -INFINITY;
+  for (int j = threadIdx.x; j < span.z; j += 256) top = fmaxf(top, p.parts.rl[slot(j)].x);
+#pragma unroll
+  for (int d = 16; d; d >>= 1) top = fmaxf(top, __shfl_xor_sync(kFullMask, top, d));
+  if (lane == 0) reach[wid] = top;
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < 8; i++) top = fmaxf(top, reach[i]);
+  const float ref = top == -INFINITY ? 0.0f : top;
+  constexpr int N = DP / 32;
+  float o[N], l = 0.0f;
+#pragma unroll
+  for (int k = 0; k < N; k++) o[k] = 0.0f;
+#pragma unroll 4
+  for (int j = wid; j < span.z; j += 8) {
+    const int64_t at = slot(j);
+    const float2 rl = p.parts.rl[at];
+    const float f = exp2_fast(rl.x - ref);
+    l += rl.y * f;
+#pragma unroll
+    for (int k = 0; k < N; k++) o[k] += p.parts.o[at * DP + lane + 32 * k] * f;
+  }
+#pragma unroll
+  for (int k = 0; k < N; k++) share[wid][lane + 32 * k] = o[k];
+  if (lane == 0) sums[wid] = l;
+  __syncthreads();
+  l = 0.0f;
+#pragma unroll
+  for (int i = 0; i < 8; i++) l += sums[i];
   const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+  const uint32_t h = (vh / p.head_tiles) * p.group + (vh % p.head_tiles) * kColumns + column;
+  T* out = static_cast<T*>(p.a.out.p) + int64_t(span.x) * p.a.out.token_stride + int64_t(h) * p.a.out.head_stride;
+  for (uint32_t d = threadIdx.x; d < p.a.c.head_dim; d += 256) {
+    float v = 0.0f;
 #pragma unroll
-  for (int j = 0; j < kMaxPerLane; j++) {
-    const uint32_t d = lane + 32 * j;
-    if (d < c.head_dim) out[d] = from_float<T>(o[j] * inv);
+    for (int i = 0; i < 8; i++) v += share[i][d];
+    out[d] = Mma<T>::from(v * inv);
   }
-  if (a.lse && lane == 0) a.lse[uint64_t(i) * a.n_q_heads + hq] = l == 0.0f ? -INFINITY : m + logf(l);
+  if (p.a.lse && threadIdx.x == 0)
+    p.a.lse[int64_t(span.x) * p.a.n_q_heads + h] = l == 0.0f ? -INFINITY : (ref + log2f(l)) * 0.6931471805599453f;
+}
+
+void check_cuda(cudaError_t e, const char* what) {
+  if (e != cudaSuccess) {
+    cudaGetLastError();
+    throw std::runtime_error(std::string(what) + ": " + cudaGetErrorString(e));
+  }
+}
+
+int sm_count() {
+  constexpr int kMaxDevices = 64;
+  static std::mutex m;
+  static int counts[kMaxDevices] = {};
+  int dev = 0;
+  check_cuda(cudaGetDevice(&dev), "get device");
+  std::lock_guard<std::mutex> lock(m);
+  if (dev >= kMaxDevices) throw std::runtime_error("device index out of range");
+  if (counts[dev] == 0) check_cuda(cudaDeviceGetAttribute(&counts[dev], cudaDevAttrMultiProcessorCount, dev), "SM count");
+  return counts[dev];
+}
+
+// Padded head dim, columns and workers of a call.
+struct Shape {
+  int dp, nt, warps;
+  uint32_t group, head_tiles, workers;
+};
+Shape shape_of(const AttendArgs& a) {
+  Shape s;
+  const uint32_t d = a.c.head_dim;
+  s.dp = d <= 64 ? 64 : d <= 96 ? 96 : d <= 128 ? 128 : 256;
+  s.group = a.n_q_heads / a.c.n_kv_heads;
+  s.nt = s.group <= 8 ? 1 : 2;
+  s.head_tiles = (s.group + 8 * s.nt - 1) / (8 * s.nt);
+  s.warps = s.dp == 64 ? 8 : 4;
+  s.workers = uint32_t(sm_count() * s.warps);
+  return s;
+}
+
+size_t aligned(size_t n) { return (n + 255) & ~size_t(255); }
+
+template <typename T, int DP, int NT>
+void launch_typed(const AttendParams& p, cudaStream_t st) {
+  constexpr int kWarps = DP == 64 ? 8 : 4, kStages = 3, TK = DP == 256 ? 16 : 32;
+  using A = Attend<T, DP, NT, TK, kWarps, kStages>;
+  auto kernel = attend_kernel<T, DP, NT, TK, kWarps, kStages>;
+  static std::mutex m;
+  static uint64_t ready = 0;  // devices where the kernel has its shared memory
+  int dev = 0;
+  check_cuda(cudaGetDevice(&dev), "get device");
+  {
+    std::lock_guard<std::mutex> lock(m);
+    if (!(ready >> dev & 1)) {
+      check_cuda(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, A::kSmem),
+                 "attend shared memory");
+      ready |= uint64_t(1) << dev;
+    }
+  }
+  if (p.parts.prefix) {
+    prefix_kernel<TK><<<1, 1024, 0, st>>>(p.a, p.parts.prefix);
+    check_cuda(cudaGetLastError(), "attend prefix launch");
+  }
+  kernel<<<p.workers / kWarps, A::kThreads, A::kSmem, st>>>(p);
+  check_cuda(cudaGetLastError(), "attend launch");
+  // rows of one tile are never split
+  if (uint64_t(p.a.c.max_pages) * p.a.c.page_size <= TK) return;
+  cudaLaunchConfig_t cfg{};
+  const uint64_t row_heads = uint64_t(p.a.n) * p.a.c.n_kv_heads * p.head_tiles;
+  cfg.gridDim = dim3(p.by_worker ? p.workers : uint32_t(row_heads), p.group < 8 * NT ? p.group : 8 * NT);
+  cfg.blockDim = dim3(256);
+  cfg.stream = st;
+  cudaLaunchAttribute attr{};
+  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr.val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = &attr;
+  cfg.numAttrs = 1;
+  check_cuda(cudaLaunchKernelEx(&cfg, join_kernel<T, DP, NT>, p), "attend join launch");
+}
+
+template <typename T>
+void launch_any(const AttendParams& p, int dp, int nt, cudaStream_t st) {
+  if (nt == 1) {
+    if (dp == 64) launch_typed<T, 64, 1>(p, st);
+    else if (dp == 96) launch_typed<T, 96, 1>(p, st);
+    else if (dp == 128) launch_typed<T, 128, 1>(p, st);
+    else launch_typed<T, 256, 1>(p, st);
+  } else {
+    if (dp == 64) launch_typed<T, 64, 2>(p, st);
+    else if (dp == 96) launch_typed<T, 96, 2>(p, st);
+    else if (dp == 128) launch_typed<T, 128, 2>(p, st);
+    else launch_typed<T, 256, 2>(p, st);
+  }
 }
 
 }  // namespace
 
-size_t attend_scratch_bytes(const AttendArgs&) { return 0; }
+size_t attend_scratch_bytes(const AttendArgs& a) {
+  if (a.n == 0 || a.n_q_heads == 0) return 0;
+  const Shape s = shape_of(a);
+  const size_t slots = size_t(2) * s.workers * 8 * s.nt;
+  return aligned(slots * s.dp * sizeof(float)) + aligned(slots * sizeof(float2)) +
+         aligned(s.workers * sizeof(int4)) + (a.n > uint32_t(kMaxListed) ? (size_t(a.n) + 1) * sizeof(int64_t) : 0);
+}
 
-void launch_attend(const AttendArgs& a, void*, cudaStream_t st) {
+void launch_attend(const AttendArgs& a, void* scratch, cudaStream_t st) {
   if (a.n == 0 || a.n_q_heads == 0) return;
-  const uint64_t blocks = uint64_t(a.n) * a.n_q_heads;
-  if (blocks > 0x7FFFFFFFull) throw std::invalid_argument("too many query heads");
-  if (a.c.dtype == JB_F16) attend_warp_kernel<__half><<<uint32_t(blocks), 32, 0, st>>>(a);
-  else attend_warp_kernel<__nv_bfloat16><<<uint32_t(blocks), 32, 0, st>>>(a);
-  const cudaError_t e = cudaGetLastError();
-  if (e != cudaSuccess)
-    throw std::runtime_error(std::string("attend launch: ") + cudaGetErrorString(e));
+  const Shape s = shape_of(a);
+  AttendParams p{};
+  p.a = a;
+  p.group = s.group;
+  p.head_tiles = s.head_tiles;
+  p.workers = s.workers;
+  const uint64_t row_heads = uint64_t(a.n) * a.c.n_kv_heads * s.head_tiles;
+  if (double(row_heads) * double(a.c.max_pages) * a.c.page_size > 4e18)
+    throw std::invalid_argument("rows, heads and tokens are too many for one call");
+  p.by_worker = row_heads > s.workers;
+  const size_t slots = size_t(2) * s.workers * 8 * s.nt;
+  unsigned char* at = static_cast<unsigned char*>(scratch);
+  p.parts.o = reinterpret_cast<float*>(at);
+  at += aligned(slots * s.dp * sizeof(float));
+  p.parts.rl = reinterpret_cast<float2*>(at);
+  at += aligned(slots * sizeof(float2));
+  p.parts.spans = reinterpret_cast<int4*>(at);
+  at += aligned(s.workers * sizeof(int4));
+  if (a.n > uint32_t(kMaxListed)) p.parts.prefix = reinterpret_cast<int64_t*>(at);
+  if (a.c.dtype == JB_F16) launch_any<__half>(p, s.dp, s.nt, st);
+  else launch_any<__nv_bfloat16>(p, s.dp, s.nt, st);
 }
 
 }  // namespace jb
