@@ -9,7 +9,7 @@
 // most 16 query heads, 2 to 32 flops a byte, so HBM.  The rest is keeping
 // enough bytes in flight and every SM equally long at work:
 //
-//  * A warp is a worker of its own.  All rows' tiles of TK tokens, one row's
+//  * A warp is a worker of its own.  All rows' tiles of 16 tokens, one row's
 //    head after the other, form one line, and worker w of W takes the w-th of
 //    W equal parts, whatever the rows' lengths.  A row's head that lies in one
 //    part is finished there; one that spans several leaves a part result in
@@ -39,6 +39,7 @@ namespace {
 
 constexpr uint32_t kFullMask = 0xFFFFFFFFu;
 constexpr int kMaxListed = 1024;  // queries whose lengths a block keeps in shared memory
+constexpr int TK = 16;            // tokens of a tile
 // A weight is 2^(s - r): r is set 6 below the largest score and stays until a
 // score is 15 above it, so weights reach 2^15, inside float16, and the largest
 // is at least 2^6: float16 weights keep 24 + 6 bits below the largest.
@@ -49,7 +50,7 @@ struct Mma;
 template <>
 struct Mma<__half> {
   static __device__ __forceinline__ void mma(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-    asm volatile(
+    asm(
         "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
         : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
         : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
@@ -67,7 +68,7 @@ struct Mma<__half> {
 template <>
 struct Mma<__nv_bfloat16> {
   static __device__ __forceinline__ void mma(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-    asm volatile(
+    asm(
         "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
         : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
         : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
@@ -95,10 +96,14 @@ __device__ __forceinline__ void ldmatrix_trans(uint32_t (&r)[4], uint32_t addr) 
 }
 __device__ __forceinline__ uint32_t transposed(uint32_t v) {
   uint32_t r;
-  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
+  asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
   return r;
 }
-// 16 bytes to shared memory, or 16 zeros
+// 16 bytes to shared memory
+__device__ __forceinline__ void copy16(uint32_t dst, const void* src) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+}
+// the same, or 16 zeros
 __device__ __forceinline__ void copy16(uint32_t dst, const void* src, bool real) {
   const int n = real ? 16 : 0;
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(n) : "memory");
@@ -132,13 +137,13 @@ struct AttendParams {
   uint32_t group, head_tiles;  // query heads of a key-value head, and tiles of 8 NT of them
   uint32_t workers;
   bool by_worker;              // what parts.spans goes by
+  bool tiled_pages;            // pages are whole tiles: a tile lies in one page
 };
 
 // The tiles of TK tokens that query i reads.
 struct Tiles {
   int32_t row, len, first, begin, end;
 };
-template <int TK>
 __device__ __forceinline__ Tiles tiles_of(const AttendArgs& a, uint32_t i) {
   Tiles t;
   t.row = a.rows ? a.rows[i] : int32_t(i);
@@ -176,14 +181,13 @@ __device__ __forceinline__ int64_t block_sum_scan(int64_t v, int64_t* total) {
 }
 
 // The tiles before each query, for more queries than a block keeps itself.
-template <int TK>
 __global__ void __launch_bounds__(1024) prefix_kernel(const AttendArgs a, int64_t* prefix) {
   int64_t done = 0;
   for (uint64_t base = 0; base < a.n; base += 1024) {
     const uint64_t i = base + threadIdx.x;
     int64_t v = 0;
     if (i < a.n) {
-      const Tiles t = tiles_of<TK>(a, uint32_t(i));
+      const Tiles t = tiles_of(a, uint32_t(i));
       v = max(t.end - t.begin, 0);
     }
     int64_t total;
@@ -192,6 +196,23 @@ __global__ void __launch_bounds__(1024) prefix_kernel(const AttendArgs a, int64_
     done += total;
   }
   if (threadIdx.x == 0) prefix[0] = 0;
+}
+
+// Warps of a block (one block an SM) and tiles of a warp's ring, for a padded
+// head dim and columns: as many bytes in flight as shared memory holds, in as
+// many warps as registers allow.
+#ifndef JB_W
+#define JB_W 12
+#define JB_S 2
+#endif
+struct Ring {
+  int warps, stages;
+};
+constexpr Ring ring_of(int DP, int NT) {
+  return DP == 64    ? Ring{12, 4}
+         : DP == 96  ? Ring{12, 2}
+         : DP == 128 ? (NT == 1 ? Ring{JB_W, JB_S} : Ring{8, 3})
+                     : Ring{6, 2};
 }
 
 // Bytes from a row of a tile in shared memory to the next.  Eight consecutive
@@ -205,6 +226,11 @@ struct TileLayout {
   static __device__ __forceinline__ uint32_t at(int row, int chunk) {
     return row * kRowBytes + (kPermuted ? (chunk ^ (row & 7)) : chunk) * 16;
   }
+  // at(row, chunk + 2 k), given at(row, chunk) in a tile on a multiple of
+  // kRowBytes, for a chunk of 0 or 1
+  static __device__ __forceinline__ uint32_t step(uint32_t addr, int k) {
+    return kPermuted ? addr ^ (32 * k) : addr + 32 * k;
+  }
 };
 
 // A place in the line of tiles: a query's head tile, and its tile.
@@ -214,7 +240,7 @@ struct Cursor {
   int32_t tile;
 };
 
-template <typename T, int DP, int NT, int TK, int WARPS, int STAGES>
+template <typename T, int DP, int NT, int WARPS, int STAGES>
 struct Attend {
   using L = TileLayout<DP>;
   static constexpr int kThreads = WARPS * 32;
@@ -224,7 +250,6 @@ struct Attend {
   static constexpr int kRingBytes = WARPS * STAGES * kStageBytes;
   static constexpr int kSmem = kRingBytes + WARPS * STAGES * 4 + kMaxListed * 8 + (kMaxListed + 1) * 8 + 8;
   static constexpr int KS = DP / 16;                     // k steps of Q K, head tiles of 16 of P V
-  static constexpr int MT = TK / 16;
   static constexpr int kChunkLanes = DP <= 64 ? 8 : DP <= 128 ? 16 : 32;  // lanes a row of 16-byte chunks takes
   static constexpr int kRowsPerCopy = 32 / kChunkLanes;
 
@@ -238,7 +263,7 @@ struct Attend {
   int lane;
 
   __device__ __forceinline__ Tiles load_tiles(uint32_t i) const {
-    if (p.parts.prefix) return tiles_of<TK>(p.a, i);
+    if (p.parts.prefix) return tiles_of(p.a, i);
     Tiles t;
     t.row = lists.row[i];
     t.len = lists.len[i];
@@ -261,41 +286,67 @@ struct Attend {
     c.tile = c.t.begin;
   }
 
-  // Page of the lane's token in a tile; -1 where it is not attended to.
-  __device__ __forceinline__ int32_t page_of(const Cursor& c, uint32_t& slot) const {
-    const int64_t t = int64_t(c.tile) * TK + lane;
-    int32_t page = -1;
-    slot = 0;
-    if (lane < TK && t >= c.t.first && t < c.t.len) {
-      const uint32_t pg = uint32_t(t) / p.a.c.page_size;
-      slot = uint32_t(t) - pg * p.a.c.page_size;
-      const bool kept = !p.a.mask || t >= p.a.mask_width || p.a.mask[int64_t(c.i) * p.a.mask_stride + t];
-      if (kept) page = p.a.c.table[c.t.row * p.a.c.table_stride + pg];
-      if (page >= 0 && uint32_t(page) >= p.a.c.n_pages) page = -1;
-    }
-    return page;
+  // Where a tile's tokens lie: the lane's token (lanes 16 on repeat lanes 0
+  // on), or with pages of whole tiles the tile's first token for all lanes.
+  struct Place {
+    int32_t page;   // -1: not there
+    uint32_t slot;
+    bool seen;      // the lane's token is attended to, if its page is there
+  };
+  __device__ __forceinline__ Place place_of(const Cursor& c) const {
+    Place x;
+    const uint32_t t = uint32_t(c.tile) * TK + (lane & 15);
+    x.seen = int32_t(t) >= c.t.first && int32_t(t) < c.t.len;
+    if (x.seen && p.a.mask && t < p.a.mask_width) x.seen = p.a.mask[int64_t(c.i) * p.a.mask_stride + t];
+    const uint32_t at = p.tiled_pages ? uint32_t(c.tile) * TK : min(t, uint32_t(c.t.len) - 1);
+    const uint32_t pg = at / p.a.c.page_size;
+    x.slot = at - pg * p.a.c.page_size;
+    x.page = p.a.c.table[c.t.row * p.a.c.table_stride + pg];
+    return x;
   }
 
-  __device__ __forceinline__ void load_tile(uint32_t stage, uint32_t* valid, const Cursor& c, int32_t page,
-                                            uint32_t slot) const {
+  __device__ __forceinline__ void load_tile(uint32_t stage, uint32_t* valid, const Cursor& c, const Place& x) const {
     const jb_page_cache& k = p.a.c;
-    const uint32_t mask = __ballot_sync(kFullMask, page >= 0);
+    const bool there = uint32_t(x.page) < k.n_pages;
+    const uint32_t mask = __ballot_sync(kFullMask, x.seen && there) & 0xFFFFu;
     if (lane == 0) *valid = mask;
-    if (mask) {
-      const int64_t base = int64_t(p.a.layer) * k.layer_stride + (c.vh / p.head_tiles) * k.head_stride;
-      const int64_t mine = base + (page >= 0 ? page * k.page_stride + slot * k.token_stride : 0);
-      const int chunk = lane % kChunkLanes;
-      const bool inside = chunk < int(k.head_dim / 8);
+    if (mask == 0) return;
+    const int chunk = lane % kChunkLanes, row0 = lane / kChunkLanes;
+    const bool inside = chunk < int(k.head_dim / 8);
+    const int64_t base = int64_t(p.a.layer) * k.layer_stride + int64_t(c.vh / p.head_tiles) * k.head_stride + chunk * 8;
+    const int64_t mine = there ? x.page * k.page_stride + x.slot * k.token_stride : 0;
+    if (p.tiled_pages) {
+      if (!inside) return;
+      const T* from = static_cast<const T*>(k.k) + base + mine + row0 * k.token_stride;
+      const int64_t to_v = static_cast<const T*>(k.v) - static_cast<const T*>(k.k);
+      const int64_t step = kRowsPerCopy * k.token_stride;
+      if (mask == 0xFFFFu) {
 #pragma unroll
-      for (int it = 0; it < TK / kRowsPerCopy; it++) {
-        const int row = it * kRowsPerCopy + lane / kChunkLanes;
-        const int64_t off = __shfl_sync(kFullMask, mine, row) + chunk * 8;
-        if (inside) {
+        for (int it = 0; it < TK / kRowsPerCopy; it++, from += step) {
+          const uint32_t dst = stage + L::at(it * kRowsPerCopy + row0, chunk);
+          copy16(dst, from);
+          copy16(dst + kTileBytes, from + to_v);
+        }
+      } else {
+#pragma unroll
+        for (int it = 0; it < TK / kRowsPerCopy; it++, from += step) {
+          const int row = it * kRowsPerCopy + row0;
           const bool real = (mask >> row) & 1;
           const uint32_t dst = stage + L::at(row, chunk);
-          copy16(dst, static_cast<const T*>(k.k) + off, real);
-          copy16(dst + kTileBytes, static_cast<const T*>(k.v) + off, real);
+          copy16(dst, real ? from : static_cast<const T*>(k.k), real);
+          copy16(dst + kTileBytes, real ? from + to_v : static_cast<const T*>(k.v), real);
         }
+      }
+    } else {
+#pragma unroll
+      for (int it = 0; it < TK / kRowsPerCopy; it++) {
+        const int row = it * kRowsPerCopy + row0;
+        const int64_t off = __shfl_sync(kFullMask, mine, row) + base;
+        if (!inside) continue;
+        const bool real = (mask >> row) & 1;
+        const uint32_t dst = stage + L::at(row, chunk);
+        copy16(dst, static_cast<const T*>(k.k) + (real ? off : 0), real);
+        copy16(dst + kTileBytes, static_cast<const T*>(k.v) + (real ? off : 0), real);
       }
     }
   }
@@ -338,41 +389,33 @@ struct Attend {
 
   __device__ __forceinline__ void tile(State& s, uint32_t stage, uint32_t mask) const {
     // S^T: rows are tokens, columns are query heads
-    float w[NT][MT][4];
+    float w[NT][4];
 #pragma unroll
-    for (int n = 0; n < NT; n++)
+    for (int n = 0; n < NT; n++) w[n][0] = w[n][1] = w[n][2] = w[n][3] = 0.0f;
+    const uint32_t keys = stage + L::at(lane & 15, lane >> 4);
 #pragma unroll
-      for (int m = 0; m < MT; m++) w[n][m][0] = w[n][m][1] = w[n][m][2] = w[n][m][3] = 0.0f;
+    for (int k = 0; k < KS; k++) {
+      uint32_t a[4];
+      ldmatrix(a, L::step(keys, k));
 #pragma unroll
-    for (int m = 0; m < MT; m++) {
-#pragma unroll
-      for (int k = 0; k < KS; k++) {
-        uint32_t a[4];
-        ldmatrix(a, stage + L::at(16 * m + (lane & 15), 2 * k + (lane >> 4)));
-#pragma unroll
-        for (int n = 0; n < NT; n++) Mma<T>::mma(w[n][m], a, s.q[n][k][0], s.q[n][k][1]);
-      }
+      for (int n = 0; n < NT; n++) Mma<T>::mma(w[n], a, s.q[n][k][0], s.q[n][k][1]);
     }
     const float scale = p.a.scale * 1.4426950408889634f;  // log2(e)
+    const bool seen0 = (mask >> (lane / 4)) & 1, seen1 = (mask >> (lane / 4 + 8)) & 1;
     bool far = false;
 #pragma unroll
     for (int n = 0; n < NT; n++)
 #pragma unroll
-      for (int m = 0; m < MT; m++)
-#pragma unroll
-        for (int j = 0; j < 4; j++) {
-          const int row = 16 * m + lane / 4 + 8 * (j / 2);
-          w[n][m][j] = (mask >> row) & 1 ? w[n][m][j] * scale : -INFINITY;
-          far |= w[n][m][j] > s.ref[n][j & 1] + kRefRoom;
-        }
+      for (int j = 0; j < 4; j++) {
+        w[n][j] = (j < 2 ? seen0 : seen1) ? w[n][j] * scale : -INFINITY;
+        far |= w[n][j] > s.ref[n][j & 1] + kRefRoom;
+      }
     if (__any_sync(kFullMask, far)) {
 #pragma unroll
       for (int n = 0; n < NT; n++)
 #pragma unroll
         for (int j = 0; j < 2; j++) {
-          float top = -INFINITY;
-#pragma unroll
-          for (int m = 0; m < MT; m++) top = fmaxf(top, fmaxf(w[n][m][j], w[n][m][j + 2]));
+          float top = fmaxf(w[n][j], w[n][j + 2]);
 #pragma unroll
           for (int d = 4; d < 32; d <<= 1) top = fmaxf(top, __shfl_xor_sync(kFullMask, top, d));
           const float ref = fmaxf(s.ref[n][j], top - kRefBelow);
@@ -387,38 +430,34 @@ struct Attend {
         }
     }
     // O^T += V^T P^T: rows are head elements
-    uint32_t hi[NT][MT][2], lo[NT][MT][2];
+    uint32_t hi[NT][2], lo[NT][2];
 #pragma unroll
     for (int n = 0; n < NT; n++) {
       const float r0 = s.ref[n][0] == -INFINITY ? 0.0f : s.ref[n][0];
       const float r1 = s.ref[n][1] == -INFINITY ? 0.0f : s.ref[n][1];
+      const float a = exp2_fast(w[n][0] - r0), b = exp2_fast(w[n][1] - r1);
+      const float c = exp2_fast(w[n][2] - r0), d = exp2_fast(w[n][3] - r1);
+      s.sum[n][0] += a + c;
+      s.sum[n][1] += b + d;
+      Mma<T>::split(a, b, hi[n][0], lo[n][0]);
+      Mma<T>::split(c, d, hi[n][1], lo[n][1]);
 #pragma unroll
-      for (int m = 0; m < MT; m++) {
-        const float a = exp2_fast(w[n][m][0] - r0), b = exp2_fast(w[n][m][1] - r1);
-        const float c = exp2_fast(w[n][m][2] - r0), d = exp2_fast(w[n][m][3] - r1);
-        s.sum[n][0] += a + c;
-        s.sum[n][1] += b + d;
-        Mma<T>::split(a, b, hi[n][m][0], lo[n][m][0]);
-        Mma<T>::split(c, d, hi[n][m][1], lo[n][m][1]);
-#pragma unroll
-        for (int j = 0; j < 2; j++) {
-          hi[n][m][j] = transposed(hi[n][m][j]);
-          lo[n][m][j] = transposed(lo[n][m][j]);
-        }
+      for (int j = 0; j < 2; j++) {
+        hi[n][j] = transposed(hi[n][j]);
+        lo[n][j] = transposed(lo[n][j]);
       }
     }
+    const uint32_t values = stage + kTileBytes + L::at((lane & 7) + ((lane >> 4) << 3), (lane >> 3) & 1);
 #pragma unroll
-    for (int m = 0; m < MT; m++)
+    for (int k = 0; k < KS; k++) {
+      uint32_t a[4];
+      ldmatrix_trans(a, L::step(values, k));
 #pragma unroll
-      for (int k = 0; k < KS; k++) {
-        uint32_t a[4];
-        ldmatrix_trans(a, stage + kTileBytes + L::at(16 * m + (lane & 7) + ((lane >> 4) << 3), 2 * k + ((lane >> 3) & 1)));
-#pragma unroll
-        for (int n = 0; n < NT; n++) {
-          Mma<T>::mma(s.o[n][k], a, hi[n][m][0], hi[n][m][1]);
-          Mma<T>::mma(s.o[n][k], a, lo[n][m][0], lo[n][m][1]);
-        }
+      for (int n = 0; n < NT; n++) {
+        Mma<T>::mma(s.o[n][k], a, hi[n][0], hi[n][1]);
+        Mma<T>::mma(s.o[n][k], a, lo[n][0], lo[n][1]);
       }
+    }
   }
 
   // The piece's end: the result, or a part of it (slot >= 0).
@@ -490,17 +529,16 @@ struct Attend {
 
     Cursor ahead = c;       // the next tile to load
     int64_t to_load = left;
-    uint32_t slot = 0;
-    int32_t page = page_of(ahead, slot);
+    Place place = place_of(ahead);
     const uint32_t stage0 = smem_addr(ring);
     int load_stage = 0;
     // loads the tile at `ahead`, and looks up the next one's pages
     auto load_next = [&] {
       if (to_load > 0) {
-        load_tile(stage0 + load_stage * kStageBytes, valid + load_stage, ahead, page, slot);
+        load_tile(stage0 + load_stage * kStageBytes, valid + load_stage, ahead, place);
         if (--to_load > 0) {
           next(ahead);
-          page = page_of(ahead, slot);
+          place = place_of(ahead);
         }
       }
       copies_commit();
@@ -549,10 +587,10 @@ struct Attend {
   }
 };
 
-template <typename T, int DP, int NT, int TK, int WARPS, int STAGES>
+template <typename T, int DP, int NT, int WARPS, int STAGES>
 __global__ void __launch_bounds__(WARPS * 32) attend_kernel(const __grid_constant__ AttendParams p) {
-  using A = Attend<T, DP, NT, TK, WARPS, STAGES>;
-  extern __shared__ __align__(128) unsigned char smem[];
+  using A = Attend<T, DP, NT, WARPS, STAGES>;
+  extern __shared__ __align__(1024) unsigned char smem[];
   uint32_t* valid = reinterpret_cast<uint32_t*>(smem + A::kRingBytes);
   int64_t* prefix = reinterpret_cast<int64_t*>(smem + ((A::kRingBytes + WARPS * STAGES * 4 + 7) & ~7));
   int32_t* row = reinterpret_cast<int32_t*>(prefix + kMaxListed + 1);
@@ -572,7 +610,7 @@ __global__ void __launch_bounds__(WARPS * 32) attend_kernel(const __grid_constan
       const uint32_t i = base + threadIdx.x;
       int64_t v = 0;
       if (i < p.a.n) {
-        const Tiles t = tiles_of<TK>(p.a, i);
+        const Tiles t = tiles_of(p.a, i);
         row[i] = t.row;
         len[i] = t.len;
         v = max(t.end - t.begin, 0);
@@ -694,7 +732,7 @@ Shape shape_of(const AttendArgs& a) {
   s.group = a.n_q_heads / a.c.n_kv_heads;
   s.nt = s.group <= 8 ? 1 : 2;
   s.head_tiles = (s.group + 8 * s.nt - 1) / (8 * s.nt);
-  s.warps = s.dp == 64 ? 8 : 4;
+  s.warps = ring_of(s.dp, s.nt).warps;
   s.workers = uint32_t(sm_count() * s.warps);
   return s;
 }
@@ -703,9 +741,9 @@ size_t aligned(size_t n) { return (n + 255) & ~size_t(255); }
 
 template <typename T, int DP, int NT>
 void launch_typed(const AttendParams& p, cudaStream_t st) {
-  constexpr int kWarps = DP == 64 ? 8 : 4, kStages = 3, TK = DP == 256 ? 16 : 32;
-  using A = Attend<T, DP, NT, TK, kWarps, kStages>;
-  auto kernel = attend_kernel<T, DP, NT, TK, kWarps, kStages>;
+  constexpr int kWarps = ring_of(DP, NT).warps, kStages = ring_of(DP, NT).stages;
+  using A = Attend<T, DP, NT, kWarps, kStages>;
+  auto kernel = attend_kernel<T, DP, NT, kWarps, kStages>;
   static std::mutex m;
   static uint64_t ready = 0;  // devices where the kernel has its shared memory
   int dev = 0;
@@ -719,7 +757,7 @@ void launch_typed(const AttendParams& p, cudaStream_t st) {
     }
   }
   if (p.parts.prefix) {
-    prefix_kernel<TK><<<1, 1024, 0, st>>>(p.a, p.parts.prefix);
+    prefix_kernel<<<1, 1024, 0, st>>>(p.a, p.parts.prefix);
     check_cuda(cudaGetLastError(), "attend prefix launch");
   }
   kernel<<<p.workers / kWarps, A::kThreads, A::kSmem, st>>>(p);
@@ -776,6 +814,7 @@ void launch_attend(const AttendArgs& a, void* scratch, cudaStream_t st) {
   if (double(row_heads) * double(a.c.max_pages) * a.c.page_size > 4e18)
     throw std::invalid_argument("rows, heads and tokens are too many for one call");
   p.by_worker = row_heads > s.workers;
+  p.tiled_pages = a.c.page_size % TK == 0;
   const size_t slots = size_t(2) * s.workers * 8 * s.nt;
   unsigned char* at = static_cast<unsigned char*>(scratch);
   p.parts.o = reinterpret_cast<float*>(at);
