@@ -40,6 +40,10 @@ namespace {
 constexpr uint32_t kFullMask = 0xFFFFFFFFu;
 constexpr int kMaxListed = 1024;  // queries whose lengths a block keeps in shared memory
 constexpr int TK = 16;            // tokens of a tile
+#ifndef JB_MIN
+#define JB_MIN 4
+#endif
+constexpr int kLeastTiles = JB_MIN;
 // A weight is 2^(s - r): r is set 6 below the largest score and stays until a
 // score is 15 above it, so weights reach 2^15, inside float16, and the largest
 // is at least 2^6: float16 weights keep 24 + 6 bits below the largest.
@@ -137,6 +141,7 @@ struct AttendParams {
   uint32_t group, head_tiles;  // query heads of a key-value head, and tiles of 8 NT of them
   uint32_t workers;
   bool by_worker;              // what parts.spans goes by
+  bool clustered;              // a cluster of blocks per row's head
   bool tiled_pages;            // pages are whole tiles: a tile lies in one page
 };
 
@@ -204,6 +209,9 @@ __global__ void __launch_bounds__(1024) prefix_kernel(const AttendArgs a, int64_
 #ifndef JB_W
 #define JB_W 12
 #define JB_S 2
+#endif
+#ifndef JB_CAP
+#define JB_CAP 4096
 #endif
 struct Ring {
   int warps, stages;
@@ -512,11 +520,13 @@ struct Attend {
   }
 
   __device__ __forceinline__ void work(uint32_t worker, unsigned char* ring, uint32_t* valid, int64_t total) const {
-    const int64_t each = total / p.workers, more = total % p.workers;
+    // a part is a few tiles at least, so that there is less to join
+    const int64_t workers = min(int64_t(p.workers), (total + kLeastTiles - 1) / kLeastTiles);
+    if (p.by_worker && lane == 0) p.parts.spans[worker] = make_int4(0, 0, 0, 0);
+    if (worker >= workers) return;
+    const int64_t each = total / workers, more = total % workers;
     const int64_t w0 = int64_t(worker) * each + min(int64_t(worker), more);
     int64_t left = each + (int64_t(worker) < more);
-    if (p.by_worker && lane == 0) p.parts.spans[worker] = make_int4(0, 0, 0, 0);
-    if (left == 0) return;
     const uint32_t heads = head_rows();
     Cursor c;
     c.i = query_at(w0 / heads);
@@ -643,6 +653,142 @@ __global__ void __launch_bounds__(WARPS * 32) attend_kernel(const __grid_constan
             total * self.head_rows());
 }
 
+// The same for few rows of few tokens, where a call's latency is what counts:
+// a cluster of kCluster blocks takes one row's head, its warps every
+// kCluster * WARPS-th tile, and the blocks' results are joined through
+// distributed shared memory, with no second kernel and no scratch.
+constexpr int kCluster = 8;
+
+template <typename T, int DP, int NT, int WARPS, int STAGES>
+__global__ void __cluster_dims__(kCluster, 1, 1) __launch_bounds__(WARPS * 32)
+attend_cluster_kernel(const __grid_constant__ AttendParams p) {
+  using A = Attend<T, DP, NT, WARPS, STAGES>;
+  constexpr int C = A::kColumns;
+  extern __shared__ __align__(1024) unsigned char smem[];
+  __shared__ uint32_t valid[WARPS * STAGES];
+  __shared__ float2 warp_rl[WARPS][C];   // a warp's references and sums
+  __shared__ float2 block_rl[C];
+  __shared__ float block_o[C][DP];
+  const int wid = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const typename A::Lists none{nullptr, nullptr, nullptr};
+  const A self{p, none, lane};
+  const uint32_t heads = self.head_rows();
+  Cursor c;
+  c.i = blockIdx.y / heads;
+  c.vh = blockIdx.y % heads;
+  typename A::State s;
+  self.begin(s, c.i, c.vh);
+  const uint32_t rank = blockIdx.x;  // the grid is one cluster wide
+  c.t = tiles_of(p.a, c.i);
+  const int count = max(c.t.end - c.t.begin, 0);
+  const int first = int(rank) * WARPS + wid, step = kCluster * WARPS;
+  unsigned char* ring = smem + wid * STAGES * A::kStageBytes;
+  if (p.a.c.head_dim < DP) {  // columns that no copy writes
+    for (int i = lane; i < STAGES * A::kStageBytes / 16; i += 32)
+      reinterpret_cast<uint4*>(ring)[i] = make_uint4(0, 0, 0, 0);
+    __syncwarp();
+  }
+  if (first < count) {
+    const uint32_t stage0 = smem_addr(ring);
+    uint32_t* mask_of = valid + wid * STAGES;
+    int to_load = first, load_stage = 0;
+    auto load_next = [&] {
+      if (to_load < count) {
+        c.tile = c.t.begin + to_load;
+        self.load_tile(stage0 + load_stage * A::kStageBytes, mask_of + load_stage, c, self.place_of(c));
+        to_load += step;
+      }
+      copies_commit();
+      load_stage = load_stage + 1 == STAGES ? 0 : load_stage + 1;
+    };
+#pragma unroll
+    for (int j = 0; j < STAGES - 1; j++) load_next();
+    int stage = 0;
+    for (int j = first; j < count; j += step) {
+      __syncwarp();
+      load_next();
+      copies_wait<STAGES - 1>();
+      __syncwarp();
+      const uint32_t mask = mask_of[stage];
+      if (mask) self.tile(s, stage0 + stage * A::kStageBytes, mask);
+      stage = stage + 1 == STAGES ? 0 : stage + 1;
+    }
+    copies_wait<0>();
+    __syncwarp();
+    // the ring is done with: it takes the warp's result
+    float* o = reinterpret_cast<float*>(ring);
+#pragma unroll
+    for (int n = 0; n < NT; n++)
+#pragma unroll
+      for (int j = 0; j < 2; j++) {
+        float l = s.sum[n][j];
+#pragma unroll
+        for (int d = 4; d < 32; d <<= 1) l += __shfl_xor_sync(kFullMask, l, d);
+        const int column = 8 * n + 2 * (lane % 4) + j;
+        if (lane < 4) warp_rl[wid][column] = make_float2(s.ref[n][j], l);
+#pragma unroll
+        for (int k = 0; k < A::KS; k++) {
+          o[column * DP + 16 * k + lane / 4] = s.o[n][k][j];
+          o[column * DP + 16 * k + lane / 4 + 8] = s.o[n][k][j + 2];
+        }
+      }
+  }
+  __syncthreads();
+  const int warps = min(WARPS, max(0, count - int(rank) * WARPS));  // those that had tiles
+  const int columns = min(C, int(p.group - (c.vh % p.head_tiles) * C));
+  for (int e = threadIdx.x; e < columns * DP; e += WARPS * 32) {
+    const int column = e / DP, d = e % DP;
+    float ref = -INFINITY;
+    for (int w = 0; w < warps; w++) ref = fmaxf(ref, warp_rl[w][column].x);
+    const float r = ref == -INFINITY ? 0.0f : ref;
+    float o = 0.0f, l = 0.0f;
+    for (int w = 0; w < warps; w++) {
+      const float2 rl = warp_rl[w][column];
+      const float f = exp2_fast(rl.x - r);
+      o += reinterpret_cast<const float*>(smem + w * STAGES * A::kStageBytes)[e] * f;
+      l += rl.y * f;
+    }
+    block_o[column][d] = o;
+    if (d == 0) block_rl[column] = make_float2(ref, l);
+  }
+  asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+  auto remote = [&](const void* at, int block) {
+    uint32_t a;
+    asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(smem_addr(at)), "r"(block));
+    return a;
+  };
+  const int dim = int(p.a.c.head_dim);
+  for (int e = int(rank) * WARPS * 32 + threadIdx.x; e < columns * DP; e += kCluster * WARPS * 32) {
+    const int column = e / DP, d = e % DP;
+    float2 rl[kCluster];
+    float part[kCluster];
+    float ref = -INFINITY;
+#pragma unroll
+    for (int b = 0; b < kCluster; b++) {
+      asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];"
+                   : "=f"(rl[b].x), "=f"(rl[b].y) : "r"(remote(&block_rl[column], b)) : "memory");
+      asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(part[b]) : "r"(remote(&block_o[column][d], b)) : "memory");
+      ref = fmaxf(ref, rl[b].x);
+    }
+    const float r = ref == -INFINITY ? 0.0f : ref;
+    float o = 0.0f, l = 0.0f;
+#pragma unroll
+    for (int b = 0; b < kCluster; b++) {
+      const float f = exp2_fast(rl[b].x - r);
+      o += part[b] * f;
+      l += rl[b].y * f;
+    }
+    const uint32_t h = self.head_of(c.vh, column);
+    if (d < dim)
+      (static_cast<T*>(p.a.out.p) + int64_t(c.i) * p.a.out.token_stride + int64_t(h) * p.a.out.head_stride)[d] =
+          Mma<T>::from(l == 0.0f ? 0.0f : o / l);
+    if (d == 0 && p.a.lse)
+      p.a.lse[int64_t(c.i) * p.a.n_q_heads + h] = l == 0.0f ? -INFINITY : (ref + log2f(l)) * 0.6931471805599453f;
+  }
+  // no block leaves while another may read its shared memory
+  asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+
 // Joins the parts of one row's head (span blockIdx.x), for one query head
 // (blockIdx.y): out = sum_i o_i 2^(r_i - r) / sum_i l_i 2^(r_i - r),
 // r the largest reference.  Eight warps take every eighth part each.
@@ -659,32 +805,51 @@ __global__ void __launch_bounds__(256) join_kernel(const __grid_constant__ Atten
   const int lane = threadIdx.x & 31, wid = threadIdx.x >> 5;
   // part 0 is the first worker's last piece, part j > 0 the next workers' first
   auto slot = [&](int j) { return (2 * (int64_t(span.w) + j) + (j == 0)) * kColumns + column; };
-  float top = -INFINITY;
-  for (int j = threadIdx.x; j < span.z; j += 256) top = fmaxf(top, p.parts.rl[slot(j)].x);
-#pragma unroll
-  for (int d = 16; d; d >>= 1) top = fmaxf(top, __shfl_xor_sync(kFullMask, top, d));
-  if (lane == 0) reach[wid] = top;
-  __syncthreads();
-#pragma unroll
-  for (int i = 0; i < 8; i++) top = fmaxf(top, reach[i]);
-  const float ref = top == -INFINITY ? 0.0f : top;
-  constexpr int N = DP / 32;
-  float o[N], l = 0.0f;
+  constexpr int N = DP / 32, B = 4;  // B parts are read at once
+  float o[N], l = 0.0f, ref = -INFINITY;
 #pragma unroll
   for (int k = 0; k < N; k++) o[k] = 0.0f;
-#pragma unroll 4
-  for (int j = wid; j < span.z; j += 8) {
-    const int64_t at = slot(j);
-    const float2 rl = p.parts.rl[at];
-    const float f = exp2_fast(rl.x - ref);
-    l += rl.y * f;
+  for (int j0 = wid; j0 < span.z; j0 += 8 * B) {
+    float2 rl[B];
+    float part[B][N];
+    float top = ref;
 #pragma unroll
-    for (int k = 0; k < N; k++) o[k] += p.parts.o[at * DP + lane + 32 * k] * f;
+    for (int b = 0; b < B; b++) {
+      const int64_t at = slot(min(j0 + 8 * b, span.z - 1));
+      rl[b] = p.parts.rl[at];
+#pragma unroll
+      for (int k = 0; k < N; k++) part[b][k] = p.parts.o[at * DP + lane + 32 * k];
+    }
+#pragma unroll
+    for (int b = 0; b < B; b++) {
+      if (j0 + 8 * b >= span.z) rl[b].x = -INFINITY;  // read twice: counts once
+      top = fmaxf(top, rl[b].x);
+    }
+    if (top == -INFINITY) continue;
+    const float keep = exp2_fast(ref - top);
+    l *= keep;
+#pragma unroll
+    for (int k = 0; k < N; k++) o[k] *= keep;
+#pragma unroll
+    for (int b = 0; b < B; b++) {
+      const float f = exp2_fast(rl[b].x - top);
+      l += rl[b].y * f;
+#pragma unroll
+      for (int k = 0; k < N; k++) o[k] += part[b][k] * f;
+    }
+    ref = top;
   }
-#pragma unroll
-  for (int k = 0; k < N; k++) share[wid][lane + 32 * k] = o[k];
-  if (lane == 0) sums[wid] = l;
+  if (lane == 0) reach[wid] = ref;
   __syncthreads();
+  float top = -INFINITY;
+#pragma unroll
+  for (int i = 0; i < 8; i++) top = fmaxf(top, reach[i]);
+  const float f = ref == -INFINITY ? 0.0f : exp2_fast(ref - top);
+#pragma unroll
+  for (int k = 0; k < N; k++) share[wid][lane + 32 * k] = o[k] * f;
+  if (lane == 0) sums[wid] = l * f;
+  __syncthreads();
+  ref = top == -INFINITY ? 0.0f : top;
   l = 0.0f;
 #pragma unroll
   for (int i = 0; i < 8; i++) l += sums[i];
@@ -724,6 +889,8 @@ int sm_count() {
 struct Shape {
   int dp, nt, warps;
   uint32_t group, head_tiles, workers;
+  uint64_t row_heads;
+  bool clustered;
 };
 Shape shape_of(const AttendArgs& a) {
   Shape s;
@@ -734,10 +901,28 @@ Shape shape_of(const AttendArgs& a) {
   s.head_tiles = (s.group + 8 * s.nt - 1) / (8 * s.nt);
   s.warps = ring_of(s.dp, s.nt).warps;
   s.workers = uint32_t(sm_count() * s.warps);
+  s.row_heads = uint64_t(a.n) * a.c.n_kv_heads * s.head_tiles;
+  // Clusters that all run at once, with rows short enough (by the table's
+  // width, or the window) that the SMs they leave idle matter less than the
+  // second kernel.
+  const uint64_t longest = uint64_t(a.c.max_pages) * a.c.page_size;
+  s.clustered = s.row_heads * kCluster <= 128 && (a.window && a.window < longest ? a.window : longest) <= JB_CAP;
   return s;
 }
 
 size_t aligned(size_t n) { return (n + 255) & ~size_t(255); }
+
+// Sets the kernel's shared memory once per device.
+template <typename K>
+void allow_shared(K kernel, int bytes, uint64_t& ready, std::mutex& m) {
+  int dev = 0;
+  check_cuda(cudaGetDevice(&dev), "get device");
+  std::lock_guard<std::mutex> lock(m);
+  if (ready >> dev & 1) return;
+  check_cuda(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes),
+             "attend shared memory");
+  ready |= uint64_t(1) << dev;
+}
 
 template <typename T, int DP, int NT>
 void launch_typed(const AttendParams& p, cudaStream_t st) {
@@ -745,17 +930,16 @@ void launch_typed(const AttendParams& p, cudaStream_t st) {
   using A = Attend<T, DP, NT, kWarps, kStages>;
   auto kernel = attend_kernel<T, DP, NT, kWarps, kStages>;
   static std::mutex m;
-  static uint64_t ready = 0;  // devices where the kernel has its shared memory
-  int dev = 0;
-  check_cuda(cudaGetDevice(&dev), "get device");
-  {
-    std::lock_guard<std::mutex> lock(m);
-    if (!(ready >> dev & 1)) {
-      check_cuda(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, A::kSmem),
-                 "attend shared memory");
-      ready |= uint64_t(1) << dev;
-    }
+  static uint64_t ready = 0, cluster_ready = 0;  // devices where the kernels have their shared memory
+  const uint64_t row_heads = uint64_t(p.a.n) * p.a.c.n_kv_heads * p.head_tiles;
+  if (p.clustered) {
+    auto cluster_kernel = attend_cluster_kernel<T, DP, NT, kWarps, kStages>;
+    allow_shared(cluster_kernel, A::kRingBytes, cluster_ready, m);
+    cluster_kernel<<<dim3(kCluster, uint32_t(row_heads)), A::kThreads, A::kRingBytes, st>>>(p);
+    check_cuda(cudaGetLastError(), "attend launch");
+    return;
   }
+  allow_shared(kernel, A::kSmem, ready, m);
   if (p.parts.prefix) {
     prefix_kernel<<<1, 1024, 0, st>>>(p.a, p.parts.prefix);
     check_cuda(cudaGetLastError(), "attend prefix launch");
@@ -765,7 +949,6 @@ void launch_typed(const AttendParams& p, cudaStream_t st) {
   // rows of one tile are never split
   if (uint64_t(p.a.c.max_pages) * p.a.c.page_size <= TK) return;
   cudaLaunchConfig_t cfg{};
-  const uint64_t row_heads = uint64_t(p.a.n) * p.a.c.n_kv_heads * p.head_tiles;
   cfg.gridDim = dim3(p.by_worker ? p.workers : uint32_t(row_heads), p.group < 8 * NT ? p.group : 8 * NT);
   cfg.blockDim = dim3(256);
   cfg.stream = st;
@@ -797,6 +980,7 @@ void launch_any(const AttendParams& p, int dp, int nt, cudaStream_t st) {
 size_t attend_scratch_bytes(const AttendArgs& a) {
   if (a.n == 0 || a.n_q_heads == 0) return 0;
   const Shape s = shape_of(a);
+  if (s.clustered) return 0;
   const size_t slots = size_t(2) * s.workers * 8 * s.nt;
   return aligned(slots * s.dp * sizeof(float)) + aligned(slots * sizeof(float2)) +
          aligned(s.workers * sizeof(int4)) + (a.n > uint32_t(kMaxListed) ? (size_t(a.n) + 1) * sizeof(int64_t) : 0);
@@ -810,10 +994,10 @@ void launch_attend(const AttendArgs& a, void* scratch, cudaStream_t st) {
   p.group = s.group;
   p.head_tiles = s.head_tiles;
   p.workers = s.workers;
-  const uint64_t row_heads = uint64_t(a.n) * a.c.n_kv_heads * s.head_tiles;
-  if (double(row_heads) * double(a.c.max_pages) * a.c.page_size > 4e18)
+  if (double(s.row_heads) * double(a.c.max_pages) * a.c.page_size > 4e18)
     throw std::invalid_argument("rows, heads and tokens are too many for one call");
-  p.by_worker = row_heads > s.workers;
+  p.by_worker = s.row_heads > s.workers;
+  p.clustered = s.clustered;
   p.tiled_pages = a.c.page_size % TK == 0;
   const size_t slots = size_t(2) * s.workers * 8 * s.nt;
   unsigned char* at = static_cast<unsigned char*>(scratch);
