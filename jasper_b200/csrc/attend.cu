@@ -40,10 +40,6 @@ namespace {
 constexpr uint32_t kFullMask = 0xFFFFFFFFu;
 constexpr int kMaxListed = 1024;  // queries whose lengths a block keeps in shared memory
 constexpr int TK = 16;            // tokens of a tile
-#ifndef JB_MIN
-#define JB_MIN 4
-#endif
-constexpr int kLeastTiles = JB_MIN;
 // A weight is 2^(s - r): r is set 6 below the largest score and stays until a
 // score is 15 above it, so weights reach 2^15, inside float16, and the largest
 // is at least 2^6: float16 weights keep 24 + 6 bits below the largest.
@@ -205,21 +201,16 @@ __global__ void __launch_bounds__(1024) prefix_kernel(const AttendArgs a, int64_
 
 // Warps of a block (one block an SM) and tiles of a warp's ring, for a padded
 // head dim and columns: as many bytes in flight as shared memory holds, in as
-// many warps as registers allow.
-#ifndef JB_W
-#define JB_W 12
-#define JB_S 2
-#endif
-#ifndef JB_CAP
-#define JB_CAP 4096
-#endif
+// many warps as their registers allow.  Measured on 400 k + 333 k tokens of 8
+// heads of 128: 12 warps with 2 tiles 447 us, 13 with 2 460, 8 with 3 467.
+// 16 query heads to a key-value head (NT 2): 8 with 3 137 us, 12 with 2 141.
 struct Ring {
   int warps, stages;
 };
 constexpr Ring ring_of(int DP, int NT) {
   return DP == 64    ? Ring{12, 4}
          : DP == 96  ? Ring{12, 2}
-         : DP == 128 ? (NT == 1 ? Ring{JB_W, JB_S} : Ring{8, 3})
+         : DP == 128 ? (NT == 1 ? Ring{12, 2} : Ring{8, 3})
                      : Ring{6, 2};
 }
 
@@ -520,8 +511,13 @@ struct Attend {
   }
 
   __device__ __forceinline__ void work(uint32_t worker, unsigned char* ring, uint32_t* valid, int64_t total) const {
-    // a part is a few tiles at least, so that there is less to join
-    const int64_t workers = min(int64_t(p.workers), (total + kLeastTiles - 1) / kLeastTiles);
+    // Parts of several tiles leave less to join, parts of one are done first.
+    // Measured on one row, 8 heads of 128, 1 / 2 / 4 tiles: 10.7 / 11.8 / 13.2
+    // us with 2000 tokens, 14.7 / 11.8 / 13.6 with 4000, 16.4 / 16.4 / 13.8
+    // with 8000.
+    const int64_t mean = total / (int64_t(p.a.n) * head_rows());
+    const int64_t least = mean < 160 ? 1 : mean < 400 ? 2 : 4;
+    const int64_t workers = min(int64_t(p.workers), (total + least - 1) / least);
     if (p.by_worker && lane == 0) p.parts.spans[worker] = make_int4(0, 0, 0, 0);
     if (worker >= workers) return;
     const int64_t each = total / workers, more = total % workers;
@@ -658,6 +654,7 @@ __global__ void __launch_bounds__(WARPS * 32) attend_kernel(const __grid_constan
 // kCluster * WARPS-th tile, and the blocks' results are joined through
 // distributed shared memory, with no second kernel and no scratch.
 constexpr int kCluster = 8;
+constexpr uint64_t kMostClusters = 15, kClusterTokens = 6000;
 
 template <typename T, int DP, int NT, int WARPS, int STAGES>
 __global__ void __cluster_dims__(kCluster, 1, 1) __launch_bounds__(WARPS * 32)
@@ -789,40 +786,47 @@ attend_cluster_kernel(const __grid_constant__ AttendParams p) {
   asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
 
-// Joins the parts of one row's head (span blockIdx.x), for one query head
-// (blockIdx.y): out = sum_i o_i 2^(r_i - r) / sum_i l_i 2^(r_i - r),
-// r the largest reference.  Eight warps take every eighth part each.
-template <typename T, int DP, int NT>
-__global__ void __launch_bounds__(256) join_kernel(const __grid_constant__ AttendParams p) {
-  constexpr int kColumns = 8 * NT;
-  __shared__ float share[8][DP];
-  __shared__ float reach[8], sums[8];
+// Joins the parts of a row's head (a span), for one query head (blockIdx.y):
+// out = sum_i o_i 2^(r_i - r) / sum_i l_i 2^(r_i - r), r the largest
+// reference.  What it takes is the latency of its dependent reads, so a warp
+// reads the references, sums and outputs of several parts at once.  With
+// few parts to a span (SHARED 1) a warp takes each, else a block of SHARED
+// warps, every SHARED-th part each.
+constexpr int kJoinSpans = 8;  // spans of a block with SHARED 1
+constexpr int join_warps(int shared) { return shared == 1 ? kJoinSpans : shared; }
+
+template <typename T, int DP, int NT, int SHARED>
+__global__ void __launch_bounds__(join_warps(SHARED) * 32) join_kernel(const __grid_constant__ AttendParams p, uint32_t spans) {
+  constexpr int kColumns = 8 * NT, N = DP / 32, B = SHARED == 16 ? 8 : 4;
+  __shared__ float share[SHARED == 1 ? 1 : SHARED][SHARED == 1 ? 1 : DP];
+  __shared__ float2 share_rl[SHARED];
+  const int lane = threadIdx.x & 31, wid = threadIdx.x >> 5;
+  const uint32_t item = SHARED == 1 ? blockIdx.x * kJoinSpans + wid : blockIdx.x;
   asm volatile("griddepcontrol.wait;" ::: "memory");
-  const int4 span = p.parts.spans[blockIdx.x];
+  if (item >= spans) return;
+  const int4 span = p.parts.spans[item];
   const int column = blockIdx.y;
   const uint32_t vh = uint32_t(span.y);
   if (span.z == 0 || (vh % p.head_tiles) * kColumns + column >= p.group) return;
-  const int lane = threadIdx.x & 31, wid = threadIdx.x >> 5;
   // part 0 is the first worker's last piece, part j > 0 the next workers' first
   auto slot = [&](int j) { return (2 * (int64_t(span.w) + j) + (j == 0)) * kColumns + column; };
-  constexpr int N = DP / 32, B = 4;  // B parts are read at once
   float o[N], l = 0.0f, ref = -INFINITY;
 #pragma unroll
   for (int k = 0; k < N; k++) o[k] = 0.0f;
-  for (int j0 = wid; j0 < span.z; j0 += 8 * B) {
+  for (int j0 = SHARED == 1 ? 0 : wid; j0 < span.z; j0 += SHARED * B) {
     float2 rl[B];
     float part[B][N];
     float top = ref;
 #pragma unroll
     for (int b = 0; b < B; b++) {
-      const int64_t at = slot(min(j0 + 8 * b, span.z - 1));
+      const int64_t at = slot(min(j0 + SHARED * b, span.z - 1));
       rl[b] = p.parts.rl[at];
 #pragma unroll
       for (int k = 0; k < N; k++) part[b][k] = p.parts.o[at * DP + lane + 32 * k];
     }
 #pragma unroll
     for (int b = 0; b < B; b++) {
-      if (j0 + 8 * b >= span.z) rl[b].x = -INFINITY;  // read twice: counts once
+      if (j0 + SHARED * b >= span.z) rl[b].x = -INFINITY;  // read twice: counts once
       top = fmaxf(top, rl[b].x);
     }
     if (top == -INFINITY) continue;
@@ -839,31 +843,37 @@ __global__ void __launch_bounds__(256) join_kernel(const __grid_constant__ Atten
     }
     ref = top;
   }
-  if (lane == 0) reach[wid] = ref;
-  __syncthreads();
-  float top = -INFINITY;
-#pragma unroll
-  for (int i = 0; i < 8; i++) top = fmaxf(top, reach[i]);
-  const float f = ref == -INFINITY ? 0.0f : exp2_fast(ref - top);
-#pragma unroll
-  for (int k = 0; k < N; k++) share[wid][lane + 32 * k] = o[k] * f;
-  if (lane == 0) sums[wid] = l * f;
-  __syncthreads();
-  ref = top == -INFINITY ? 0.0f : top;
-  l = 0.0f;
-#pragma unroll
-  for (int i = 0; i < 8; i++) l += sums[i];
-  const float inv = l == 0.0f ? 0.0f : 1.0f / l;
   const uint32_t h = (vh / p.head_tiles) * p.group + (vh % p.head_tiles) * kColumns + column;
   T* out = static_cast<T*>(p.a.out.p) + int64_t(span.x) * p.a.out.token_stride + int64_t(h) * p.a.out.head_stride;
-  for (uint32_t d = threadIdx.x; d < p.a.c.head_dim; d += 256) {
-    float v = 0.0f;
+  float* lse = p.a.lse ? p.a.lse + int64_t(span.x) * p.a.n_q_heads + h : nullptr;
+  if constexpr (SHARED == 1) {
+    const float inv = l == 0.0f ? 0.0f : 1.0f / l;
 #pragma unroll
-    for (int i = 0; i < 8; i++) v += share[i][d];
-    out[d] = Mma<T>::from(v * inv);
+    for (int k = 0; k < N; k++)
+      if (lane + 32 * k < p.a.c.head_dim) out[lane + 32 * k] = Mma<T>::from(o[k] * inv);
+    if (lse && lane == 0) *lse = l == 0.0f ? -INFINITY : (ref + log2f(l)) * 0.6931471805599453f;
+  } else {
+#pragma unroll
+    for (int k = 0; k < N; k++) share[wid][lane + 32 * k] = o[k];
+    if (lane == 0) share_rl[wid] = make_float2(ref, l);
+    __syncthreads();
+    float top = -INFINITY;
+#pragma unroll
+    for (int i = 0; i < SHARED; i++) top = fmaxf(top, share_rl[i].x);
+    const float r = top == -INFINITY ? 0.0f : top;
+    for (uint32_t d = threadIdx.x; d < p.a.c.head_dim; d += SHARED * 32) {
+      float v = 0.0f;
+      l = 0.0f;
+#pragma unroll
+      for (int i = 0; i < SHARED; i++) {
+        const float f = exp2_fast(share_rl[i].x - r);
+        v += share[i][d] * f;
+        l += share_rl[i].y * f;
+      }
+      out[d] = Mma<T>::from(l == 0.0f ? 0.0f : v / l);
+      if (lse && d == 0) *lse = l == 0.0f ? -INFINITY : (top + log2f(l)) * 0.6931471805599453f;
+    }
   }
-  if (p.a.lse && threadIdx.x == 0)
-    p.a.lse[int64_t(span.x) * p.a.n_q_heads + h] = l == 0.0f ? -INFINITY : (ref + log2f(l)) * 0.6931471805599453f;
 }
 
 void check_cuda(cudaError_t e, const char* what) {
@@ -902,11 +912,13 @@ Shape shape_of(const AttendArgs& a) {
   s.warps = ring_of(s.dp, s.nt).warps;
   s.workers = uint32_t(sm_count() * s.warps);
   s.row_heads = uint64_t(a.n) * a.c.n_kv_heads * s.head_tiles;
-  // Clusters that all run at once, with rows short enough (by the table's
-  // width, or the window) that the SMs they leave idle matter less than the
-  // second kernel.
+  // Few enough clusters that all run at once (15 of 8 do here, 16 do not: 7.5
+  // and 13 us), and rows short enough, by the table's width or the window,
+  // that the SMs they leave idle matter less than the second kernel.  One row,
+  // 8 heads of 128, clusters / equal parts: 7.2 / 10.0 us with 1000 tokens,
+  // 10.2 / 12.0 with 4000, 14.5 / 13.8 with 8000.
   const uint64_t longest = uint64_t(a.c.max_pages) * a.c.page_size;
-  s.clustered = s.row_heads * kCluster <= 128 && (a.window && a.window < longest ? a.window : longest) <= JB_CAP;
+  s.clustered = s.row_heads <= kMostClusters && (a.window && a.window < longest ? a.window : longest) <= kClusterTokens;
   return s;
 }
 
@@ -948,16 +960,22 @@ void launch_typed(const AttendParams& p, cudaStream_t st) {
   check_cuda(cudaGetLastError(), "attend launch");
   // rows of one tile are never split
   if (uint64_t(p.a.c.max_pages) * p.a.c.page_size <= TK) return;
+  const uint32_t spans = p.by_worker ? p.workers : uint32_t(row_heads);
+  const uint32_t parts = p.workers / spans;  // about as many to a span
+  const int shared = parts >= 48 ? 16 : parts >= 6 ? 4 : 1;
   cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3(p.by_worker ? p.workers : uint32_t(row_heads), p.group < 8 * NT ? p.group : 8 * NT);
-  cfg.blockDim = dim3(256);
+  cfg.gridDim = dim3(shared == 1 ? (spans + kJoinSpans - 1) / kJoinSpans : spans, p.group < 8 * NT ? p.group : 8 * NT);
+  cfg.blockDim = dim3(join_warps(shared) * 32);
   cfg.stream = st;
   cudaLaunchAttribute attr{};
   attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr.val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = &attr;
   cfg.numAttrs = 1;
-  check_cuda(cudaLaunchKernelEx(&cfg, join_kernel<T, DP, NT>, p), "attend join launch");
+  auto join = shared == 16  ? join_kernel<T, DP, NT, 16>
+              : shared == 4 ? join_kernel<T, DP, NT, 4>
+                            : join_kernel<T, DP, NT, 1>;
+  check_cuda(cudaLaunchKernelEx(&cfg, join, p, spans), "attend join launch");
 }
 
 template <typename T>
