@@ -59,7 +59,7 @@ const jb_page_cache& checked(const jb_page_cache* c) {
           "head_dim must be a multiple of 8, at most 256");
   require(c->page_size > 0 && c->page_size <= (1u << 20), "page_size must be 1 to 2^20");
   require(c->n_kv_heads > 0 && c->n_kv_heads <= 65536, "n_kv_heads must be 1 to 65536");
-  require(c->n_pages < (1u << 30), "n_pages must be below 2^30");
+  require(c->n_pages < (1u << 29), "n_pages must be below 2^29");
   require(c->n_rows < (1u << 30) && c->max_pages < (1u << 30), "n_rows and max_pages must be below 2^30");
   require(c->table && c->lengths && c->refs && c->status, "null pointer in the cache");
   require((c->k && c->v) || c->n_pages == 0 || c->n_layers == 0, "null pointer in the cache");

@@ -3,6 +3,7 @@
 //
 // Every choice is by number, never by arrival: free pages are taken lowest
 // first, in the order of the rows that ask, so equal states give equal tables.
+#include <mutex>
 #include <stdexcept>
 #include <string>
 #include "paged.cuh"
@@ -11,6 +12,12 @@ namespace jb {
 namespace {
 
 constexpr int kPlanThreads = 1024;
+constexpr int kPlanBlocks = 8;           // one cluster; a pool of one block's pages takes one block
+constexpr int kThreadPages = 16;         // a thread's pages, next to each other
+constexpr uint32_t kBlockPages = kPlanThreads * kThreadPages;
+constexpr uint32_t kRowsInBlock = 2048;  // rows of a call, and of the table, whose book-keeping
+constexpr uint32_t kOwnersInBlock = 8192;  // a block keeps in its shared memory
+constexpr size_t kPlanShared = 4 * kRowsInBlock * 4 + kOwnersInBlock * 4 + kBlockPages * 2;
 
 void check_launch(const char* what) {
   const cudaError_t e = cudaGetLastError();
@@ -23,6 +30,11 @@ __device__ __forceinline__ bool row_ok(const jb_page_cache& c, int32_t r) {
 }
 __device__ __forceinline__ bool page_ok(const jb_page_cache& c, int32_t p) {
   return p >= 0 && uint32_t(p) < c.n_pages;
+}
+
+// Pages of up to 2^31 tokens.
+__device__ __forceinline__ uint32_t pages_for(uint32_t tokens, uint32_t page_size) {
+  return (tokens + page_size - 1) / page_size;
 }
 
 // Sums of pages saturate here: far above any pool, and two of them fit an int.
@@ -57,151 +69,304 @@ __device__ __forceinline__ int block_scan(int v, int* total) {
   return min(before + x, kManyPages);
 }
 
-// Scratch of a plan over n rows: owner[n_rows], need[n], upto[n], from[n]
-// (fork: the page to copy), fill[n] (fork: its tokens), page[n_pages].
-struct Plan {
-  int32_t *owner, *have, *need, *upto, *from, *free_list;
-  __host__ __device__ Plan(int32_t* s, const jb_page_cache& c, uint64_t n)
-      : owner(s), have(s + c.n_rows), need(have + n), upto(need + n), from(upto + n),
-        free_list(from + n) {}
+// ── plans ────────────────────────────────────────────────────────────────
+// extend, fork and compact decide over the whole pool at once, in one cluster
+// of blocks: block r looks at the r-th part of the pages, the blocks' counts
+// meet in distributed shared memory, and then every page knows its rank.  What
+// a call names (rows, in order) every block works out for itself, in its own
+// shared memory, or where that is too small in its own part of the scratch.
+// Latency is what bounds them: a few dependent reads and two cluster barriers.
+// One block that walked the pool 1024 pages at a time took 45 us for 65,536.
+// A pool that one block sees in one turn takes one block, without barriers.
+
+__device__ __forceinline__ uint32_t cluster_rank() {
+  uint32_t r;
+  asm("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+  return r;
+}
+template <int BLOCKS>
+__device__ __forceinline__ void cluster_arrive() {
+  if (BLOCKS > 1) asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+}
+template <int BLOCKS>
+__device__ __forceinline__ void cluster_wait() {
+  if (BLOCKS > 1) asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+  else __syncthreads();
+}
+
+// Every block's `mine`, exchanged: *before gets the sum over the blocks below
+// this one; returns the sum over all.  `box` is BLOCKS ints of shared memory
+// of its own for each exchange of a kernel.  All threads call it, and have
+// waited for the barrier that every block arrives at first: only then have all
+// blocks started, and may be written to.
+template <int BLOCKS>
+__device__ __forceinline__ int exchange(int mine, int* box, int* before) {
+  *before = 0;
+  if (BLOCKS == 1) {
+    __syncthreads();
+    return mine;
+  }
+  const uint32_t rank = cluster_rank();
+  if (threadIdx.x < BLOCKS) {
+    uint32_t at;
+    asm("mapa.shared::cluster.u32 %0, %1, %2;"
+        : "=r"(at) : "r"(static_cast<uint32_t>(__cvta_generic_to_shared(box + rank))), "r"(threadIdx.x));
+    asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(at), "r"(mine) : "memory");
+  }
+  cluster_arrive<BLOCKS>();
+  cluster_wait<BLOCKS>();
+  int all = 0;
+#pragma unroll
+  for (int i = 0; i < BLOCKS; i++) {
+    if (i < int(rank)) *before = min(*before + box[i], kManyPages);
+    all = min(all + box[i], kManyPages);
+  }
+  return all;
+}
+
+// The block's part of the pool, and the pages of a thread's turn in it.
+struct PoolPart {
+  uint32_t begin, end;
+  __device__ __forceinline__ PoolPart(const jb_page_cache& c, uint32_t blocks) {
+    const uint32_t each = (c.n_pages + blocks * kThreadPages - 1) / (blocks * kThreadPages) * kThreadPages;
+    begin = min(cluster_rank() * each, c.n_pages);
+    end = min(begin + each, c.n_pages);
+  }
+  __device__ __forceinline__ uint32_t turns() const { return (end - begin + kBlockPages - 1) / kBlockPages; }
+  __device__ __forceinline__ uint32_t first(uint32_t turn) const {
+    return begin + turn * kBlockPages + threadIdx.x * kThreadPages;
+  }
 };
 
-// owner[row] = the first i that names the row.
-__device__ void claim_rows(const jb_page_cache& c, const int32_t* rows, uint32_t n, int32_t* owner) {
-  for (uint32_t r = threadIdx.x; r < c.n_rows; r += blockDim.x) owner[r] = 0x7FFFFFFF;
-  __syncthreads();
-  for (uint32_t i = threadIdx.x; i < n; i += blockDim.x)
-    if (row_ok(c, rows[i])) atomicMin(owner + rows[i], int32_t(i));
-  __syncthreads();
-}
-
-// The lowest `total` free pages, in order, into list; returns how many there are.
-__device__ int lowest_free(const jb_page_cache& c, int total, int32_t* list) {
-  int found = 0;
-  for (uint64_t base = 0; base < c.n_pages && found < total; base += blockDim.x) {
-    const uint64_t p = base + threadIdx.x;
-    const int is = p < c.n_pages && c.refs[p] == 0;
-    int sum;
-    const int rank = found + block_scan(is, &sum) - 1;
-    if (is && rank < total) list[rank] = int32_t(p);
-    found += sum;
+// Which of the thread's pages from `first` on are free, as bits.
+__device__ __forceinline__ uint32_t free_bits(const jb_page_cache& c, const PoolPart& part, uint32_t first) {
+  uint32_t bits = 0;
+  if (first + kThreadPages <= part.end && (reinterpret_cast<uintptr_t>(c.refs) & 15) == 0) {
+    int4 v[kThreadPages / 4];
+#pragma unroll
+    for (int i = 0; i < kThreadPages / 4; i++) v[i] = reinterpret_cast<const int4*>(c.refs + first)[i];
+#pragma unroll
+    for (int i = 0; i < kThreadPages / 4; i++)
+      bits |= ((v[i].x <= 0) | (v[i].y <= 0) << 1 | (v[i].z <= 0) << 2 | (v[i].w <= 0) << 3) << (4 * i);
+  } else {
+    for (uint32_t i = 0; i < kThreadPages && first + i < part.end; i++) bits |= (c.refs[first + i] <= 0) << i;
   }
-  __syncthreads();
-  return min(found, total);
+  return bits;
 }
 
-// need[i] pages wanted by row i (0 for those refused), in order: upto[i] is
-// their running sum.  Returns the total.
-__device__ int sum_needs(uint32_t n, const int32_t* need, int32_t* upto) {
-  int total = 0;
-  for (uint32_t base = 0; base < n; base += blockDim.x) {
-    const uint32_t i = base + threadIdx.x;
-    const int v = i < n ? need[i] : 0;
-    int sum;
-    const int incl = block_scan(v, &sum);
-    if (i < n) upto[i] = min(total + incl, kManyPages);
-    total = min(total + sum, kManyPages);
+// A call's rows as a block keeps them: the row, what it has, the pages that it
+// and those before it want (saturating), and more.
+struct Wants {
+  int32_t *owner, *row, *have, *upto, *extra;
+  uint16_t* free_list;
+  __device__ Wants(const jb_page_cache& c, uint32_t n, unsigned char* shared, int32_t* scratch) {
+    int32_t* mem = reinterpret_cast<int32_t*>(shared);
+    scratch += size_t(cluster_rank()) * (size_t(c.n_rows) + 4 * size_t(n));
+    owner = c.n_rows <= kOwnersInBlock ? mem + 4 * kRowsInBlock : scratch;
+    free_list = reinterpret_cast<uint16_t*>(mem + 4 * kRowsInBlock + kOwnersInBlock);
+    const bool fits = n <= kRowsInBlock;
+    int32_t* lists = fits ? mem : scratch + c.n_rows;
+    const size_t step = fits ? kRowsInBlock : n;
+    row = lists;
+    have = lists + step;
+    upto = lists + 2 * step;
+    extra = lists + 3 * step;
   }
-  __syncthreads();
-  return total;
+  __device__ void clear(const jb_page_cache& c) {
+    for (uint32_t r = threadIdx.x; r < c.n_rows; r += blockDim.x) owner[r] = 0x7FFFFFFF;
+    __syncthreads();
+  }
+  // owner[row] = the first i that names the row
+  __device__ void claim(uint32_t i, int32_t r, bool ok) {
+    row[i] = r;
+    if (ok) atomicMin(owner + r, int32_t(i));
+  }
+  // upto holds what each row wants, and then the running sum; returns the total
+  __device__ int sum(uint32_t n) {
+    int total = 0;
+    for (uint32_t base = 0; base < n; base += blockDim.x) {
+      const uint32_t i = base + threadIdx.x;
+      const int v = i < n ? upto[i] : 0;
+      int all;
+      const int incl = block_scan(v, &all);
+      if (i < n) upto[i] = min(total + incl, kManyPages);
+      total = min(total + all, kManyPages);
+    }
+    __syncthreads();
+    return total;
+  }
+  // the row that the rank-th new page goes to: the first with upto > rank
+  __device__ uint32_t row_of(int rank, uint32_t n) const {
+    uint32_t low = 0, high = n - 1;
+    while (low < high) {
+      const uint32_t mid = (low + high) / 2;
+      if (upto[mid] > rank) high = mid;
+      else low = mid + 1;
+    }
+    return low;
+  }
+};
+
+// Finds the lowest free pages and calls give(rank, page) for each rank below
+// `total`; `bits0` are the thread's free pages of its first turn, `before` the
+// free pages of the blocks below.  The pages go through a list (kBlockPages
+// entries), so that each is a thread's of its own: a thread that gave its 16
+// away one by one took 4 us.
+template <typename F>
+__device__ __forceinline__ void hand_out(const jb_page_cache& c, const PoolPart& part, uint32_t bits0, int before,
+                                         int total, uint16_t* list, F&& give) {
+  for (uint32_t turn = 0; turn < part.turns() && before < total; turn++) {
+    const uint32_t first = part.first(turn), base = part.begin + turn * kBlockPages;
+    uint32_t bits = turn == 0 ? bits0 : free_bits(c, part, first);
+    int all;
+    const int n = __popc(bits);
+    int at = block_scan(n, &all) - n;
+    for (; bits; bits &= bits - 1) list[at++] = uint16_t(first - base + __ffs(bits) - 1);
+    __syncthreads();
+    for (int i = threadIdx.x; i < min(all, total - before); i += kPlanThreads)
+      give(before + i, int32_t(base + list[i]));
+    __syncthreads();
+    before += all;
+  }
 }
 
-__global__ void __launch_bounds__(kPlanThreads)
-extend_kernel(const jb_page_cache c, const int32_t* rows, const int32_t* tokens, uint32_t n,
-              int32_t* scratch) {
-  const Plan s(scratch, c, n);
-  claim_rows(c, rows, n, s.owner);
-  const int64_t ps = c.page_size;
+// The thread's free pages of its first turn, and the block's count of all.
+__device__ __forceinline__ int count_free(const jb_page_cache& c, const PoolPart& part, uint32_t bits0) {
+  int n = __popc(bits0);
+  for (uint32_t turn = 1; turn < part.turns(); turn++) n += __popc(free_bits(c, part, part.first(turn)));
+  int all;
+  block_scan(n, &all);
+  return all;
+}
+
+template <int BLOCKS>
+__global__ void __cluster_dims__(BLOCKS, 1, 1) __launch_bounds__(kPlanThreads)
+extend_kernel(const jb_page_cache c, const int32_t* rows, const int32_t* tokens, uint32_t n, int32_t* scratch) {
+  extern __shared__ __align__(16) unsigned char shared[];
+  __shared__ int box[BLOCKS];
+  cluster_arrive<BLOCKS>();
+  const PoolPart part(c, BLOCKS);
+  const uint32_t bits = free_bits(c, part, part.first(0));
+  Wants w(c, n, shared, scratch);
+  // A turn of rows: what they name and have, read before anything waits.
+  struct Turn {
+    int32_t r = -1, more = -1, len = 0;
+    __device__ Turn(const jb_page_cache& c, const int32_t* rows, const int32_t* tokens, uint32_t i, uint32_t n) {
+      if (i >= n) return;
+      r = rows[i];
+      more = tokens[i];
+      if (row_ok(c, r)) len = max(c.lengths[r], 0);
+    }
+  };
+  const Turn first(c, rows, tokens, threadIdx.x, n);
+  w.clear(c);
   for (uint32_t i = threadIdx.x; i < n; i += blockDim.x) {
-    const int32_t r = rows[i], more = tokens[i];
-    int need = -1, have = 0;
-    if (row_ok(c, r) && s.owner[r] == int32_t(i) && more >= 0) {
-      const int64_t len = max(c.lengths[r], 0);
-      have = int((len + ps - 1) / ps);
-      const int64_t want = (len + more + ps - 1) / ps;
-      if (want <= c.max_pages && len + more <= 0x7FFFFFFF) need = max(int(want) - have, 0);
-    }
-    if (need < 0) atomicOr(c.status, kPagesBadRow);
-    s.have[i] = need < 0 ? -1 : have;
-    s.need[i] = max(need, 0);
+    const Turn t = i == threadIdx.x ? first : Turn(c, rows, tokens, i, n);
+    w.claim(i, t.r, row_ok(c, t.r));
+    w.have[i] = t.len;
+    w.extra[i] = t.more;
   }
   __syncthreads();
-  const int total = min(sum_needs(n, s.need, s.upto), int(c.n_pages));
-  const int n_free = lowest_free(c, total, s.free_list);
-  const int lane = threadIdx.x & 31;
-  for (uint32_t i = threadIdx.x >> 5; i < n; i += blockDim.x >> 5) {
-    if (s.have[i] < 0) continue;
-    const int need = s.need[i], upto = s.upto[i];
-    if (need > 0 && upto > n_free) {
-      if (lane == 0) atomicOr(c.status, kPagesExhausted);
-      continue;
-    }
-    int32_t* row = c.table + rows[i] * c.table_stride + s.have[i];
-    for (int j = lane; j < need; j += 32) {
-      const int32_t p = s.free_list[upto - need + j];
-      row[j] = p;
-      c.refs[p] = 1;
-    }
-    if (lane == 0) c.lengths[rows[i]] = max(c.lengths[rows[i]], 0) + tokens[i];
+  const bool speaks = cluster_rank() == 0;  // one block sets status bits and lengths
+  for (uint32_t i = threadIdx.x; i < n; i += blockDim.x) {
+    const int32_t r = w.row[i], more = w.extra[i];
+    const uint32_t len = uint32_t(w.have[i]), sum = len + uint32_t(max(more, 0));
+    const uint32_t have = pages_for(len, c.page_size), pages = pages_for(sum, c.page_size);
+    const bool ok = row_ok(c, r) && w.owner[r] == int32_t(i) && more >= 0 && sum <= 0x7FFFFFFFu && pages <= c.max_pages;
+    if (!ok && speaks) atomicOr(c.status, kPagesBadRow);
+    w.have[i] = ok ? int32_t(have) : -1;
+    w.upto[i] = ok && pages > have ? int32_t(pages - have) : 0;
+    w.extra[i] = ok ? int32_t(sum) : -1;  // the row's length behind the call
+  }
+  __syncthreads();
+  const int total = w.sum(n);
+  int before;
+  cluster_wait<BLOCKS>();
+  const int n_free = exchange<BLOCKS>(count_free(c, part, bits), box, &before);  // all lengths are read behind this
+  hand_out(c, part, bits, before, min(total, n_free), w.free_list, [&](int rank, int32_t page) {
+    const uint32_t i = w.row_of(rank, n);
+    if (w.upto[i] > n_free) return;
+    const int into = rank - (i ? w.upto[i - 1] : 0);
+    c.table[w.row[i] * c.table_stride + w.have[i] + into] = page;
+    c.refs[page] = 1;
+  });
+  if (!speaks) return;
+  for (uint32_t i = threadIdx.x; i < n; i += blockDim.x) {
+    if (w.have[i] < 0) continue;
+    const bool none = pages_for(uint32_t(w.extra[i]), c.page_size) <= uint32_t(w.have[i]);
+    if (none || w.upto[i] <= n_free) c.lengths[w.row[i]] = w.extra[i];
+    else atomicOr(c.status, kPagesExhausted);
   }
 }
 
-__global__ void __launch_bounds__(kPlanThreads)
-fork_kernel(const jb_page_cache c, const int32_t* parents, const int32_t* children, uint32_t n,
+// copies: from[n], to[n] (-1: none), tokens[n], length[n] (-1: pair refused);
+// the copying kernel shares the whole pages
+template <int BLOCKS>
+__global__ void __cluster_dims__(BLOCKS, 1, 1) __launch_bounds__(kPlanThreads)
+fork_kernel(const jb_page_cache c, const int32_t* parents, const int32_t* children, uint32_t n, int32_t* copies,
             int32_t* scratch) {
-  const Plan s(scratch, c, n);
-  claim_rows(c, children, n, s.owner);
-  const int32_t ps = int32_t(c.page_size);
-  for (uint32_t i = threadIdx.x; i < n; i += blockDim.x) {
-    const int32_t p = parents[i], ch = children[i];
-    int32_t len = -1, from = -1;
-    if (row_ok(c, p) && row_ok(c, ch) && s.owner[ch] == int32_t(i) && c.lengths[ch] == 0) {
-      len = max(c.lengths[p], 0);
-      if (uint32_t((int64_t(len) + ps - 1) / ps) > c.max_pages) {
-        len = -1;
-      } else if (len % ps) {
-        from = c.table[p * c.table_stride + len / ps];
-        if (!page_ok(c, from)) from = -1;
-      }
+  extern __shared__ __align__(16) unsigned char shared[];
+  __shared__ int box[BLOCKS];
+  cluster_arrive<BLOCKS>();
+  const PoolPart part(c, BLOCKS);
+  const uint32_t bits = free_bits(c, part, part.first(0));
+  Wants w(c, n, shared, scratch);
+  struct Turn {
+    int32_t child = -1, len = -1, from = -1;  // len -1: no pair to fork
+    __device__ Turn(const jb_page_cache& c, const int32_t* parents, const int32_t* children, uint32_t i, uint32_t n) {
+      if (i >= n) return;
+      const int32_t p = parents[i];
+      child = children[i];
+      const int32_t there = row_ok(c, child) ? c.lengths[child] : -1;
+      const int32_t held = row_ok(c, p) ? max(c.lengths[p], 0) : -1;
+      if (there != 0 || held < 0 || pages_for(uint32_t(held), c.page_size) > c.max_pages) return;
+      len = held;
+      const uint32_t whole = uint32_t(len) / c.page_size;
+      if (whole * c.page_size == uint32_t(len)) return;
+      from = c.table[p * c.table_stride + whole];
+      if (!page_ok(c, from)) from = -1;
     }
-    if (len < 0) atomicOr(c.status, kPagesBadRow);
-    s.have[i] = len;
-    s.from[i] = from;
-    s.need[i] = from >= 0;
+  };
+  const Turn first(c, parents, children, threadIdx.x, n);
+  w.clear(c);
+  for (uint32_t i = threadIdx.x; i < n; i += blockDim.x) {
+    const Turn t = i == threadIdx.x ? first : Turn(c, parents, children, i, n);
+    w.claim(i, t.child, row_ok(c, t.child));
+    w.have[i] = t.len;
+    w.extra[i] = t.from;
   }
   __syncthreads();
-  const int total = min(sum_needs(n, s.need, s.upto), int(c.n_pages));
-  const int n_free = lowest_free(c, total, s.free_list);
-  const int lane = threadIdx.x & 31;
-  for (uint32_t i = threadIdx.x >> 5; i < n; i += blockDim.x >> 5) {
-    const int32_t len = s.have[i];
-    const bool given = len >= 0 && (s.need[i] == 0 || s.upto[i] <= n_free);
-    int32_t page = -1;
-    if (!given) {
-      if (lane == 0 && len >= 0) atomicOr(c.status, kPagesExhausted);
-    } else {
-      const int32_t* src = c.table + parents[i] * c.table_stride;
-      int32_t* dst = c.table + children[i] * c.table_stride;
-      const int whole = len / ps;
-      for (int j = lane; j < whole; j += 32) {
-        const int32_t p = src[j];
-        const bool ok = page_ok(c, p);
-        dst[j] = ok ? p : -1;
-        if (ok) atomicAdd(c.refs + p, 1);
-      }
-      if (s.need[i]) page = s.free_list[s.upto[i] - 1];
-      if (lane == 0) {
-        if (len % ps) dst[whole] = page;
-        if (page >= 0) c.refs[page] = 1;
-        c.lengths[children[i]] = len;
-      }
+  const bool speaks = cluster_rank() == 0;
+  int32_t *from_of = copies, *to_of = copies + n, *tokens_of = to_of + n, *length_of = tokens_of + n;
+  for (uint32_t i = threadIdx.x; i < n; i += blockDim.x) {
+    if (w.have[i] >= 0 && w.owner[w.row[i]] != int32_t(i)) w.have[i] = w.extra[i] = -1;
+    const int32_t len = w.have[i], from = w.extra[i];
+    w.upto[i] = from >= 0;
+    if (speaks) {
+      if (len < 0) atomicOr(c.status, kPagesBadRow);
+      from_of[i] = from;
+      to_of[i] = -1;
+      tokens_of[i] = from >= 0 ? int32_t(uint32_t(len) % c.page_size) : 0;
     }
-    // what the copies read: from[i] -> upto[i], need[i] tokens
-    __syncwarp();
-    if (lane == 0) {
-      s.upto[i] = page;
-      s.need[i] = page >= 0 ? len % ps : 0;
-    }
+  }
+  __syncthreads();
+  const int total = w.sum(n);
+  int before;
+  cluster_wait<BLOCKS>();
+  const int n_free = exchange<BLOCKS>(count_free(c, part, bits), box, &before);  // rows are read, and copies set, behind this
+  hand_out(c, part, bits, before, min(total, n_free), w.free_list, [&](int rank, int32_t page) {
+    const uint32_t i = w.row_of(rank, n);
+    c.table[w.row[i] * c.table_stride + uint32_t(w.have[i]) / c.page_size] = page;
+    c.refs[page] = 1;
+    to_of[i] = page;
+  });
+  if (!speaks) return;
+  for (uint32_t i = threadIdx.x; i < n; i += blockDim.x) {
+    const int32_t len = w.have[i];
+    const bool given = len >= 0 && (w.extra[i] < 0 || w.upto[i] <= n_free);
+    length_of[i] = given ? len : -1;
+    if (given) c.lengths[w.row[i]] = len;
+    else if (len >= 0) atomicOr(c.status, kPagesExhausted);
   }
 }
 
@@ -223,9 +388,13 @@ free_kernel(const jb_page_cache c, const int32_t* rows, uint32_t n) {
   if (threadIdx.x == 0) c.lengths[r] = 0;
 }
 
+// owner[row] = the first i that names the row
 __global__ void __launch_bounds__(kPlanThreads)
 adopt_claim_kernel(const jb_page_cache c, const int32_t* rows, uint32_t n, int32_t* owner) {
-  claim_rows(c, rows, n, owner);
+  for (uint32_t r = threadIdx.x; r < c.n_rows; r += blockDim.x) owner[r] = 0x7FFFFFFF;
+  __syncthreads();
+  for (uint32_t i = threadIdx.x; i < n; i += blockDim.x)
+    if (row_ok(c, rows[i])) atomicMin(owner + rows[i], int32_t(i));
 }
 
 __global__ void __launch_bounds__(128)
@@ -255,102 +424,218 @@ adopt_kernel(const jb_page_cache c, const int32_t* rows, const int32_t* pages, i
 }
 
 // moves[0]: how many; then the pages that move and, n_pages on, where to.
-__global__ void __launch_bounds__(kPlanThreads)
+template <int BLOCKS>
+__global__ void __cluster_dims__(BLOCKS, 1, 1) __launch_bounds__(kPlanThreads)
 compact_plan_kernel(const jb_page_cache c, int32_t* remap, int32_t* moves) {
-  int n_live = 0;
-  for (uint64_t base = 0; base < c.n_pages; base += blockDim.x) {
-    const uint64_t p = base + threadIdx.x;
-    int sum;
-    block_scan(p < c.n_pages && c.refs[p] > 0, &sum);
-    n_live += sum;
+  __shared__ int live_box[BLOCKS], hole_box[BLOCKS], mover_box[BLOCKS];
+  cluster_arrive<BLOCKS>();
+  const PoolPart part(c, BLOCKS);
+  const uint32_t bits0 = free_bits(c, part, part.first(0));
+  int unused;
+  const int free_here = count_free(c, part, bits0);
+  cluster_wait<BLOCKS>();
+  const int n_live = exchange<BLOCKS>(int(part.end - part.begin) - free_here, live_box, &unused);
+  // of the thread's pages from `first` on: holes, free and below n_live, and
+  // movers, live and at or above it
+  auto split = [&](uint32_t first, uint32_t bits, uint32_t* holes, uint32_t* movers) {
+    const int inside = min(max(int(part.end) - int(first), 0), kThreadPages);
+    const int below = min(max(n_live - int(first), 0), inside);
+    *holes = bits & ((1u << below) - 1);
+    *movers = ~bits & ((1u << inside) - 1) & ~((1u << below) - 1);
+  };
+  int n_holes = 0, n_movers = 0;
+  for (uint32_t turn = 0; turn < part.turns(); turn++) {
+    uint32_t holes, movers;
+    split(part.first(turn), turn == 0 ? bits0 : free_bits(c, part, part.first(turn)), &holes, &movers);
+    n_holes += __popc(holes);
+    n_movers += __popc(movers);
   }
+  int holes_here, movers_here, holes_before, movers_before;
+  block_scan(n_holes, &holes_here);
+  block_scan(n_movers, &movers_here);
+  exchange<BLOCKS>(holes_here, hole_box, &holes_before);
+  const int n_moves = exchange<BLOCKS>(movers_here, mover_box, &movers_before);
   int32_t* src = moves + 1;
   int32_t* dst = src + c.n_pages;
-  int holes = 0, movers = 0;
-  for (uint64_t base = 0; base < c.n_pages; base += blockDim.x) {
-    const uint64_t p = base + threadIdx.x;
-    const bool in = p < c.n_pages;
-    const bool live = in && c.refs[p] > 0;
-    const int hole = in && !live && int64_t(p) < n_live, mover = live && int64_t(p) >= n_live;
-    int sum;
-    const int hr = block_scan(hole, &sum);
-    if (hole) dst[holes + hr - 1] = int32_t(p);
-    holes += sum;
-    const int mr = block_scan(mover, &sum);
-    if (mover) src[movers + mr - 1] = int32_t(p);
-    movers += sum;
-    if (in) remap[p] = live ? int32_t(p) : -1;
+  for (uint32_t turn = 0; turn < part.turns(); turn++) {
+    const uint32_t first = part.first(turn);
+    const uint32_t bits = turn == 0 ? bits0 : free_bits(c, part, first);
+    uint32_t holes, movers;
+    split(first, bits, &holes, &movers);
+    int all, at = holes_before + block_scan(__popc(holes), &all) - __popc(holes);
+    holes_before += all;
+    for (uint32_t m = holes; m; m &= m - 1) dst[at++] = int32_t(first + __ffs(m) - 1);
+    at = movers_before + block_scan(__popc(movers), &all) - __popc(movers);
+    movers_before += all;
+    for (uint32_t m = movers; m; m &= m - 1) src[at++] = int32_t(first + __ffs(m) - 1);
+    for (uint32_t i = 0; i < kThreadPages && first + i < part.end; i++)
+      if (!(movers >> i & 1)) remap[first + i] = bits >> i & 1 ? -1 : int32_t(first + i);
   }
-  __syncthreads();
-  for (int j = threadIdx.x; j < movers; j += blockDim.x) {
+  if (cluster_rank() == 0 && threadIdx.x == 0) moves[0] = n_moves;
+  cluster_arrive<BLOCKS>();
+  cluster_wait<BLOCKS>();
+  for (int j = cluster_rank() * kPlanThreads + threadIdx.x; j < n_moves; j += BLOCKS * kPlanThreads) {
     remap[src[j]] = dst[j];
     c.refs[dst[j]] = c.refs[src[j]];
     c.refs[src[j]] = 0;
   }
-  if (threadIdx.x == 0) moves[0] = movers;
 }
 
-__global__ void __launch_bounds__(256) remap_table_kernel(const jb_page_cache c, const int32_t* remap) {
-  const uint64_t total = uint64_t(c.n_rows) * c.max_pages;
-  for (uint64_t i = uint64_t(blockIdx.x) * blockDim.x + threadIdx.x; i < total;
-       i += uint64_t(gridDim.x) * blockDim.x) {
-    int32_t* e = c.table + int64_t(i / c.max_pages) * c.table_stride + i % c.max_pages;
-    const int32_t p = *e;
-    if (p >= 0) *e = page_ok(c, p) ? remap[p] : -1;
+// ── copies ───────────────────────────────────────────────────────────────
+// Pages src[i] -> dst[i] in keys, values and every layer, tokens[i] tokens of
+// each (null: all); n pairs, or *n_device.  HBM bounds it: a warp takes 4 KB
+// of one page of one plane at a time, eight 16-byte reads of each lane before
+// the first write.  On the way, with `remap` the rows' table is rewritten, and
+// with `parents` the whole pages of forked rows are shared.
+constexpr int kCopyThreads = 256, kCopyDepth = 8;
+
+struct CopyArgs {
+  jb_page_cache c;
+  const int32_t *src, *dst, *tokens;
+  uint32_t n;
+  const int32_t* n_device;
+  const int32_t* remap;
+  const int32_t *parents, *children, *lengths;
+  // a page's tokens lie as runs: `flat`, all in one run; `by_head`, a run for
+  // each head; else a run for each token and head
+  bool flat, by_head;
+};
+
+__global__ void __launch_bounds__(kCopyThreads) copy_pages_kernel(const __grid_constant__ CopyArgs a) {
+  const jb_page_cache& c = a.c;
+  if (a.remap) {
+    const uint64_t total = uint64_t(c.n_rows) * c.max_pages;
+    for (uint64_t i = uint64_t(blockIdx.x) * kCopyThreads + threadIdx.x; i < total; i += uint64_t(gridDim.x) * kCopyThreads) {
+      int32_t* e = c.table + int64_t(i / c.max_pages) * c.table_stride + i % c.max_pages;
+      const int32_t p = *e;
+      if (p >= 0) *e = page_ok(c, p) ? a.remap[p] : -1;
+    }
   }
-}
-
-// Copies of pages src[i] -> dst[i] in keys, values and every layer, tokens[i]
-// tokens of each (null: all); n pairs, or *n_device.
-__global__ void __launch_bounds__(256)
-copy_pages_kernel(const jb_page_cache c, const int32_t* src, const int32_t* dst,
-                  const int32_t* tokens, uint32_t n, const int32_t* n_device) {
-  const uint32_t pairs = n_device ? uint32_t(max(*n_device, 0)) : n;
-  const uint32_t planes = 2 * c.n_layers;
-  const uint32_t chunks = c.head_dim / 8;  // 16 bytes each
-  for (uint64_t item = blockIdx.x; item < uint64_t(pairs) * planes; item += gridDim.x) {
-    const uint32_t i = uint32_t(item / planes), plane = uint32_t(item % planes);
-    const int32_t from = src[i], to = dst[i];
+  const uint32_t lane = threadIdx.x & 31;
+  const uint64_t step = uint64_t(gridDim.x) * (kCopyThreads / 32);
+  const uint64_t warp = uint64_t(blockIdx.x) * (kCopyThreads / 32) + threadIdx.x / 32;
+  if (a.parents)
+    for (uint64_t i = warp; i < a.n; i += step) {
+      const int32_t len = a.lengths[i], whole = len / int32_t(c.page_size);
+      if (len < 0) continue;
+      const int32_t* from = c.table + a.parents[i] * c.table_stride;
+      int32_t* to = c.table + a.children[i] * c.table_stride;
+      for (int j = lane; j < whole; j += 32) {
+        const int32_t p = from[j];
+        const bool ok = page_ok(c, p);
+        to[j] = ok ? p : -1;
+        if (ok) atomicAdd(c.refs + p, 1);
+      }
+      if (lane == 0 && len % int32_t(c.page_size) && a.src[i] < 0) to[whole] = -1;
+    }
+  const uint32_t pairs = a.n_device ? uint32_t(max(*a.n_device, 0)) : a.n;
+  const uint32_t planes = 2 * c.n_layers, row = c.head_dim / 8;  // 16-byte vectors of a head
+  const uint32_t full = c.page_size * c.n_kv_heads * row;
+  const uint32_t pieces = (full + 32 * kCopyDepth - 1) / (32 * kCopyDepth);
+  const uint64_t units = uint64_t(pairs) * planes * pieces;
+  for (uint64_t unit = warp; unit < units; unit += step) {
+    const uint64_t item = unit / pieces;
+    const uint32_t piece = uint32_t(unit - item * pieces);
+    const uint32_t i = uint32_t(item / planes), plane = uint32_t(item - uint64_t(i) * planes);
+    const int32_t from = a.src[i], to = a.dst[i];
     if (!page_ok(c, from) || !page_ok(c, to)) {
-      if (threadIdx.x == 0 && !tokens) atomicOr(c.status, kPagesBadToken);
+      if (lane == 0 && !a.tokens) atomicOr(c.status, kPagesBadToken);
       continue;
     }
-    uint16_t* base = static_cast<uint16_t*>(plane & 1 ? c.v : c.k) + (plane >> 1) * c.layer_stride;
+    const uint32_t nt = a.tokens ? uint32_t(a.tokens[i]) : c.page_size;
+    const uint32_t count = nt * c.n_kv_heads * row;
+    const uint32_t v0 = piece * 32 * kCopyDepth + lane;
+    uint16_t* base = static_cast<uint16_t*>(plane & 1 ? c.v : c.k) + int64_t(plane >> 1) * c.layer_stride;
     const uint16_t* s = base + from * c.page_stride;
     uint16_t* d = base + to * c.page_stride;
-    const uint32_t nt = tokens ? uint32_t(tokens[i]) : c.page_size;
-    for (uint32_t u = threadIdx.x; u < nt * c.n_kv_heads * chunks; u += blockDim.x) {
-      const uint32_t th = u / chunks, e = u % chunks;
-      const int64_t off = (th / c.n_kv_heads) * c.token_stride + (th % c.n_kv_heads) * c.head_stride + e * 8;
-      *reinterpret_cast<uint4*>(d + off) = *reinterpret_cast<const uint4*>(s + off);
+    uint4 v[kCopyDepth];
+    int64_t off[kCopyDepth];
+#pragma unroll
+    for (int k = 0; k < kCopyDepth; k++) {
+      const uint32_t u = v0 + 32 * k;
+      if (a.flat) {
+        off[k] = int64_t(u) * 8;
+      } else if (a.by_head) {
+        const uint32_t h = u / (nt * row);
+        off[k] = int64_t(h) * c.head_stride + int64_t(u - h * nt * row) * 8;
+      } else {
+        const uint32_t th = u / row, t = th / c.n_kv_heads;
+        off[k] = int64_t(t) * c.token_stride + int64_t(th - t * c.n_kv_heads) * c.head_stride + int64_t(u - th * row) * 8;
+      }
+      if (u < count) v[k] = *reinterpret_cast<const uint4*>(s + off[k]);
     }
+#pragma unroll
+    for (int k = 0; k < kCopyDepth; k++)
+      if (v0 + 32 * k < count) *reinterpret_cast<uint4*>(d + off[k]) = v[k];
   }
 }
 
-uint32_t copy_grid(uint64_t items) { return uint32_t(items < 148 * 8 ? (items ? items : 1) : 148 * 8); }
+void launch_copies(CopyArgs a, cudaStream_t st) {
+  const jb_page_cache& c = a.c;
+  const int64_t dim = c.head_dim, heads = c.n_kv_heads, ps = c.page_size;
+  const bool token_rows = c.head_stride == dim && c.token_stride == heads * dim;  // a token's heads, then the next token
+  a.by_head = c.token_stride == dim;
+  a.flat = token_rows || (a.by_head && a.tokens == nullptr && c.head_stride == ps * dim);
+  const uint64_t full = uint64_t(c.page_size) * c.n_kv_heads * (c.head_dim / 8);
+  if (full > 0x7FFFFFFFull) throw std::invalid_argument("a page is too large");
+  const uint64_t units = uint64_t(a.n) * 2 * c.n_layers * ((full + 32 * kCopyDepth - 1) / (32 * kCopyDepth));
+  const uint64_t blocks = (units + kCopyThreads / 32 - 1) / (kCopyThreads / 32);
+  constexpr uint64_t kMost = 148 * 8;
+  copy_pages_kernel<<<uint32_t(blocks < kMost ? (blocks ? blocks : 1) : kMost), kCopyThreads, 0, st>>>(a);
+  check_launch("copy pages");
+}
+
+// Launches a plan kernel; its shared memory is allowed once per device.
+template <auto Kernel, int BLOCKS, typename... A>
+void launch_plan_of(const char* what, cudaStream_t st, A... args) {
+  static std::mutex m;
+  static uint64_t ready = 0;
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess) check_launch(what);
+  {
+    std::lock_guard<std::mutex> lock(m);
+    if (!(ready >> dev & 1)) {
+      if (cudaFuncSetAttribute(Kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, int(kPlanShared)) != cudaSuccess)
+        check_launch(what);
+      ready |= uint64_t(1) << dev;
+    }
+  }
+  Kernel<<<BLOCKS, kPlanThreads, kPlanShared, st>>>(args...);
+  check_launch(what);
+}
+#define JB_LAUNCH_PLAN(kernel, what, c, ...)                                                    \
+  do {                                                                                          \
+    if ((c).n_pages <= kBlockPages) launch_plan_of<kernel<1>, 1>(what, __VA_ARGS__);            \
+    else launch_plan_of<kernel<kPlanBlocks>, kPlanBlocks>(what, __VA_ARGS__);                   \
+  } while (0)
 
 }  // namespace
 
 size_t pages_plan_words(const jb_page_cache& c, uint64_t n) {
-  return size_t(c.n_rows) + 4 * size_t(n) + 2 * size_t(c.n_pages) + 1;
+  const size_t lists = c.n_rows > kOwnersInBlock || n > kRowsInBlock ? kPlanBlocks * (size_t(c.n_rows) + 4 * size_t(n)) : 0;
+  return lists + 4 * size_t(n) + 2 * size_t(c.n_pages) + 1;
 }
 
 void launch_extend(const jb_page_cache& c, const int32_t* rows, const int32_t* tokens, uint32_t n,
                    int32_t* scratch, cudaStream_t st) {
   if (n == 0) return;
-  extend_kernel<<<1, kPlanThreads, 0, st>>>(c, rows, tokens, n, scratch);
-  check_launch("extend");
+  JB_LAUNCH_PLAN(extend_kernel, "extend", c, st, c, rows, tokens, n, scratch);
 }
 
 void launch_fork(const jb_page_cache& c, const int32_t* parents, const int32_t* children, uint32_t n,
                  int32_t* scratch, cudaStream_t st) {
   if (n == 0) return;
-  fork_kernel<<<1, kPlanThreads, 0, st>>>(c, parents, children, n, scratch);
-  check_launch("fork");
-  const Plan s(scratch, c, n);
-  copy_pages_kernel<<<copy_grid(uint64_t(n) * 2 * c.n_layers), 256, 0, st>>>(c, s.from, s.upto, s.need, n,
-                                                                            nullptr);
-  check_launch("fork copy");
+  JB_LAUNCH_PLAN(fork_kernel, "fork", c, st, c, parents, children, n, scratch, scratch + 4 * size_t(n));
+  CopyArgs a{};
+  a.c = c;
+  a.n = n;
+  a.src = scratch;
+  a.dst = a.src + n;
+  a.tokens = a.dst + n;
+  a.lengths = a.tokens + n;
+  a.parents = parents;
+  a.children = children;
+  launch_copies(a, st);
 }
 
 void launch_free(const jb_page_cache& c, const int32_t* rows, uint32_t n, cudaStream_t st) {
@@ -371,21 +656,26 @@ void launch_adopt(const jb_page_cache& c, const int32_t* rows, const int32_t* pa
 
 void launch_compact(const jb_page_cache& c, int32_t* remap, int32_t* scratch, cudaStream_t st) {
   if (c.n_pages == 0) return;
-  compact_plan_kernel<<<1, kPlanThreads, 0, st>>>(c, remap, scratch);
-  check_launch("compact");
-  remap_table_kernel<<<148 * 4, 256, 0, st>>>(c, remap);
-  check_launch("compact table");
-  copy_pages_kernel<<<copy_grid(uint64_t(c.n_pages) * 2 * c.n_layers), 256, 0, st>>>(
-      c, scratch + 1, scratch + 1 + c.n_pages, nullptr, 0, scratch);
-  check_launch("compact copy");
+  JB_LAUNCH_PLAN(compact_plan_kernel, "compact", c, st, c, remap, scratch);
+  CopyArgs a{};
+  a.c = c;
+  a.n = c.n_pages;
+  a.n_device = scratch;
+  a.src = scratch + 1;
+  a.dst = a.src + c.n_pages;
+  a.remap = remap;
+  launch_copies(a, st);
 }
 
 void launch_copy_pages(const jb_page_cache& c, const int32_t* src, const int32_t* dst, uint32_t n,
                        cudaStream_t st) {
   if (n == 0) return;
-  copy_pages_kernel<<<copy_grid(uint64_t(n) * 2 * c.n_layers), 256, 0, st>>>(c, src, dst, nullptr, n,
-                                                                            nullptr);
-  check_launch("copy pages");
+  CopyArgs a{};
+  a.c = c;
+  a.n = n;
+  a.src = src;
+  a.dst = dst;
+  launch_copies(a, st);
 }
 
 }  // namespace jb
