@@ -390,7 +390,8 @@ typedef struct jb_page_cache {
  * a turn: products with whole positions wrap at whole turns, so angles are
  * exact to float32 for every int64 position.  `inverse` turns backwards: the
  * gradient with respect to x, given y's.  x and y: [n_tokens][n_heads]
- * [head_dim] of `dtype` at any token and head stride (elements); y may be x.
+ * [head_dim] of `dtype` at any token and head stride (elements), head_dim at
+ * most 512; y may be x.
  * positions: n_tokens int32, or int64 with positions_64.  Runs on the current
  * device. */
 int jb_rotary(const void* x, int64_t x_token_stride, int64_t x_head_stride, void* y,

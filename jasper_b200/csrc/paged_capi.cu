@@ -110,8 +110,7 @@ int jb_rotary(const void* x, int64_t x_token_stride, int64_t x_head_stride, void
               int32_t inverse, void* stream) {
   return jb::capi_guarded([&] {
     require(dtype == JB_F16 || dtype == JB_BF16 || dtype == JB_F32, "dtype must be JB_F16, JB_BF16 or JB_F32");
-    require(head_dim > 0 && head_dim <= 65536, "head_dim must be 1 to 65536");
-    require(rot_dim <= 8192, "rot_dim must be at most 8192");
+    require(head_dim > 0 && head_dim <= 512, "head_dim must be 1 to 512");
     require(n_heads <= 65536, "n_heads must be at most 65536");
     if (n_tokens == 0 || n_heads == 0) return;
     require(x && y && positions && freq, "null pointer argument");

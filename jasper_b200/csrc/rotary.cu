@@ -8,10 +8,14 @@
 // 32 bits of the product are the reduced angle, exact for every int64
 // position; only then does it become a float32 (error 2^-25 of a turn).
 //
-// A block takes a few tokens: it first computes their cosines and sines once
-// (half a head of pairs each, shared by all heads) into shared memory, then
-// streams the tokens' heads through registers, two vectors of a pair's two
-// sides at a time.
+// HBM bounds prompts, latency single tokens.  A block takes a few tokens: it
+// computes their cosines and sines once (half a head of pairs each, shared by
+// all heads) into shared memory while its first heads are on their way, then
+// streams the tokens' heads through registers, two 16-byte vectors of a pair's
+// two sides at a time.  A thread keeps its place in the head, so nothing is
+// divided on the way.  One pair of vectors a thread in flight and 1536 threads
+// an SM beat more of them in fewer threads: 8192 tokens of 40 heads of 128 in
+// bfloat16 took 31 us so, 34 and 48 with two and four in flight.
 #include <stdexcept>
 #include <string>
 #include "paged.cuh"
@@ -19,8 +23,9 @@
 namespace jb {
 namespace {
 
-constexpr int kThreads = 256;
-constexpr int kMaxTokens = 16;  // per block
+constexpr int kMaxThreads = 256;  // a block has as many whole heads' units as fit
+constexpr int kMaxTokens = 16;    // per block
+constexpr int kBlocks = 6;        // of 256 threads an SM, by registers
 
 template <typename T>
 struct Elem;
@@ -48,6 +53,8 @@ struct alignas(sizeof(T) * VEC) Vec {
 struct RotaryParams {
   HeadsView q, q_out, k, v;  // q alone for jb_rotary
   uint32_t n_q, n_kv, dim, tokens_per_block;
+  uint32_t units;      // of a head: pairs of vectors
+  bool stream;         // results are more than L2 keeps: write them through
   uint64_t n_tokens;
   Positions pos;
   RotaryArgs r;
@@ -59,32 +66,87 @@ struct RotaryParams {
 };
 
 template <typename T, int VEC, bool APPEND>
-__global__ void __launch_bounds__(kThreads) rotary_kernel(const RotaryParams a) {
-  extern __shared__ float2 cs[];  // [tokens][rot / 2]
+__global__ void __launch_bounds__(kMaxThreads, kBlocks) rotary_kernel(const __grid_constant__ RotaryParams a) {
+  extern __shared__ float2 cs[];  // [tokens][VEC][rot / 2 / VEC]: neighbouring threads read neighbours
   __shared__ int64_t place[kMaxTokens];
-  const uint32_t half = a.r.rot / 2;
+  using V = Vec<T, VEC>;
+  const uint32_t half = a.r.rot / 2, pair_units = half / VEC;
   const uint64_t t0 = uint64_t(blockIdx.x) * a.tokens_per_block;
   const uint32_t nt = uint32_t(min(uint64_t(a.tokens_per_block), a.n_tokens - t0));
+  const uint32_t heads = a.n_q + (APPEND ? 2 * a.n_kv : 0);
+  const uint32_t e = threadIdx.x % a.units, stride = blockDim.x / a.units;
+  const bool turn = e < pair_units;
+  // the unit's two vectors in its head
+  const uint32_t o0 = turn ? (a.r.interleaved ? 2 * VEC * e : VEC * e) : a.r.rot + 2 * VEC * (e - pair_units);
+  const uint32_t o1 = turn && !a.r.interleaved ? o0 + half : o0 + VEC;
+  const bool two = o1 < a.dim;
+
+  // heads of the block's tokens, one after the other
+  struct Head {
+    uint32_t tok, h;
+  };
+  auto from = [&](const Head& x) {
+    const uint64_t t = t0 + x.tok;
+    uint32_t h = x.h;
+    const HeadsView* v = &a.q;
+    if (APPEND && h >= a.n_q) {
+      h -= a.n_q;
+      v = &a.k;
+      if (h >= a.n_kv) {
+        h -= a.n_kv;
+        v = &a.v;
+      }
+    }
+    return static_cast<const T*>(v->p) + t * v->token_stride + h * v->head_stride;
+  };
+  auto advance = [&](Head& x) {
+    x.h += stride;
+    while (x.h >= heads) {
+      x.h -= heads;
+      x.tok++;
+    }
+  };
+  Head at{0, threadIdx.x / a.units};
+  while (at.h >= heads) {
+    at.h -= heads;
+    at.tok++;
+  }
+  V x0, x1;
+  auto load = [&] {
+    const T* src = from(at);
+    x0 = *reinterpret_cast<const V*>(src + o0);
+    if (two) x1 = *reinterpret_cast<const V*>(src + o1);
+  };
+  auto store = [&](T* dst, const V& v) {
+    if constexpr (sizeof(V) == 16) {
+      if (a.stream) {
+        __stcs(reinterpret_cast<uint4*>(dst), *reinterpret_cast<const uint4*>(&v));
+        return;
+      }
+    }
+    *reinterpret_cast<V*>(dst) = v;
+  };
+  if (at.tok < nt) load();
 
   if (APPEND && threadIdx.x < nt) {
     // the token's place in its page, -1 where there is none
     const uint64_t t = t0 + threadIdx.x;
     const int32_t row = a.rows[t];
-    int64_t at = -1;
+    int64_t to = -1;
     if (row >= 0 && uint32_t(row) < a.c.n_rows) {
       const int64_t i = a.index ? int64_t(a.index[t]) : int64_t(a.c.lengths[row]) - 1;
-      if (i >= 0 && uint64_t(i) / a.c.page_size < a.c.max_pages) {
+      if (i >= 0 && uint32_t(i) / a.c.page_size < a.c.max_pages) {
         const uint32_t pg = uint32_t(i) / a.c.page_size, slot = uint32_t(i) % a.c.page_size;
         const int32_t page = a.c.table[row * a.c.table_stride + pg];
         if (page >= 0 && uint32_t(page) < a.c.n_pages)
-          at = a.layer_offset + page * a.c.page_stride + slot * a.c.token_stride;
+          to = a.layer_offset + page * a.c.page_stride + slot * a.c.token_stride;
       }
     }
-    place[threadIdx.x] = at;
-    if (at < 0) atomicOr(a.c.status, kPagesBadToken);
+    place[threadIdx.x] = to;
+    if (to < 0) atomicOr(a.c.status, kPagesBadToken);
   }
-  for (uint32_t j = threadIdx.x; j < nt * half; j += kThreads) {
-    const uint32_t tok = j / half, i = j % half;
+  for (uint32_t j = threadIdx.x; j < nt * half; j += blockDim.x) {
+    const uint32_t tok = j / half, i = j - tok * half;
     const uint64_t t = t0 + tok;
     int64_t p;
     if (!APPEND || a.pos.p32 || a.pos.p64) {
@@ -98,52 +160,30 @@ __global__ void __launch_bounds__(kThreads) rotary_kernel(const RotaryParams a) 
     const uint64_t phase = uint64_t(p) * uint64_t(a.r.freq[i]);
     float sn, cn;
     sincospif(float(int32_t(phase >> 32)) * 0x1p-31f, &sn, &cn);
-    cs[j] = make_float2(cn * a.r.scale, (a.r.inverse ? -sn : sn) * a.r.scale);
+    cs[tok * half + (i % VEC) * pair_units + i / VEC] = make_float2(cn * a.r.scale, (a.r.inverse ? -sn : sn) * a.r.scale);
   }
   __syncthreads();
 
-  const uint32_t pair_units = half / VEC;
-  const uint32_t units = pair_units + (a.dim - a.r.rot + 2 * VEC - 1) / (2 * VEC);
-  const uint32_t heads = a.n_q + (APPEND ? 2 * a.n_kv : 0);
-  using V = Vec<T, VEC>;
-  for (uint32_t u = threadIdx.x; u < nt * heads * units; u += kThreads) {
-    const uint32_t hu = u / units, e = u % units;
-    const uint32_t tok = hu / heads;
-    uint32_t h = hu % heads;
-    const uint64_t t = t0 + tok;
-    const T* src;
+  for (; at.tok < nt; advance(at)) {
+    if (at.tok || at.h >= stride) load();  // the first is there
+    const uint64_t t = t0 + at.tok;
     T* dst;
-    bool turn = e < pair_units, plain_head = false;
-    if (h < a.n_q) {
-      src = static_cast<const T*>(a.q.p) + t * a.q.token_stride + h * a.q.head_stride;
-      dst = static_cast<T*>(a.q_out.p) + t * a.q_out.token_stride + h * a.q_out.head_stride;
+    bool turned = turn;
+    if (!APPEND || at.h < a.n_q) {
+      dst = static_cast<T*>(a.q_out.p) + t * a.q_out.token_stride + at.h * a.q_out.head_stride;
     } else {
-      if (place[tok] < 0) continue;
-      h -= a.n_q;
-      const bool is_k = h < a.n_kv;
-      if (!is_k) h -= a.n_kv;
-      const HeadsView& s = is_k ? a.k : a.v;
-      src = static_cast<const T*>(s.p) + t * s.token_stride + h * s.head_stride;
-      dst = static_cast<T*>(is_k ? a.c.k : a.c.v) + place[tok] + h * a.c.head_stride;
-      plain_head = !is_k;
+      if (place[at.tok] < 0) continue;
+      const bool is_k = at.h - a.n_q < a.n_kv;
+      const uint32_t h = at.h - a.n_q - (is_k ? 0 : a.n_kv);
+      dst = static_cast<T*>(is_k ? a.c.k : a.c.v) + place[at.tok] + h * a.c.head_stride;
+      turned = turn && is_k;
     }
-    uint32_t o0, o1;  // the unit's two vectors
-    if (turn) {
-      o0 = a.r.interleaved ? 2 * VEC * e : VEC * e;
-      o1 = a.r.interleaved ? o0 + VEC : o0 + half;
-    } else {
-      o0 = a.r.rot + 2 * VEC * (e - pair_units);
-      o1 = o0 + VEC;
-    }
-    const bool two = o1 < a.dim;
-    V x0 = *reinterpret_cast<const V*>(src + o0), x1;
-    if (two) x1 = *reinterpret_cast<const V*>(src + o1);
-    if (turn && !plain_head) {
-      const float2* c = cs + tok * half + VEC * e;
+    if (turned) {
+      const float2* c = cs + at.tok * half + e;
       if (a.r.interleaved) {
 #pragma unroll
         for (int i = 0; i < VEC; i++) {  // pair i: elements 2i, 2i + 1 of the two vectors
-          const float2 w = c[i];
+          const float2 w = c[i * pair_units];
           T& ra = 2 * i < VEC ? x0.v[(2 * i) % VEC] : x1.v[(2 * i) % VEC];
           T& rb = 2 * i + 1 < VEC ? x0.v[(2 * i + 1) % VEC] : x1.v[(2 * i + 1) % VEC];
           const float fa = Elem<T>::to(ra), fb = Elem<T>::to(rb);
@@ -153,15 +193,15 @@ __global__ void __launch_bounds__(kThreads) rotary_kernel(const RotaryParams a) 
       } else {
 #pragma unroll
         for (int i = 0; i < VEC; i++) {
-          const float2 w = c[i];
+          const float2 w = c[i * pair_units];
           const float fa = Elem<T>::to(x0.v[i]), fb = Elem<T>::to(x1.v[i]);
           x0.v[i] = Elem<T>::from(fa * w.x - fb * w.y);
           x1.v[i] = Elem<T>::from(fb * w.x + fa * w.y);
         }
       }
     }
-    *reinterpret_cast<V*>(dst + o0) = x0;
-    if (two) *reinterpret_cast<V*>(dst + o1) = x1;
+    store(dst + o0, x0);
+    if (two) store(dst + o1, x1);
   }
 }
 
@@ -198,18 +238,29 @@ void launch_typed(RotaryParams a, cudaStream_t st) {
   const uint32_t heads = a.n_q + (APPEND ? 2 * a.n_kv : 0);
   if (heads == 0) return;
   const int vec = w.vec(sizeof(T));
-  a.tokens_per_block = 1;
+  a.units = a.r.rot / 2 / vec + (a.dim - a.r.rot + 2 * vec - 1) / (2 * vec);
+  // Many tokens go two to a block, few get a block each, for their latency.
+  // Two tokens of many heads stay longer in 128 threads than in 256 and hide
+  // more (40 heads of 128: 28.9 and 29.8 us for 8192 tokens); of few heads
+  // they would take more turns (12 heads of 80: 7.3 and 6.2 us for 4099).
+  const bool many = a.n_tokens >= 1024;
+  a.tokens_per_block = many ? 2 : 1;
+  const bool half_block = many && a.units <= kMaxThreads / 2 && 2 * uint64_t(a.units) * heads >= 2 * kMaxThreads;
+  const uint32_t most = half_block ? kMaxThreads / 2 : kMaxThreads;
+  const uint32_t threads = most / a.units * a.units;
+  a.stream = a.n_tokens * heads * a.dim * sizeof(T) > (uint64_t(32) << 20);
   const uint64_t blocks = (a.n_tokens + a.tokens_per_block - 1) / a.tokens_per_block;
   if (blocks > 0x7FFFFFFFull) throw std::invalid_argument("too many tokens");
   const size_t smem = size_t(a.tokens_per_block) * (a.r.rot / 2) * sizeof(float2);
-  switch (vec) {
-    case 8:
-      if constexpr (sizeof(T) == 2)
-        rotary_kernel<T, 8, APPEND><<<uint32_t(blocks), kThreads, smem, st>>>(a);
-      break;
-    case 4: rotary_kernel<T, 4, APPEND><<<uint32_t(blocks), kThreads, smem, st>>>(a); break;
-    case 2: rotary_kernel<T, 2, APPEND><<<uint32_t(blocks), kThreads, smem, st>>>(a); break;
-    default: rotary_kernel<T, 1, APPEND><<<uint32_t(blocks), kThreads, smem, st>>>(a); break;
+  auto launch = [&](auto kernel) { kernel<<<uint32_t(blocks), threads, smem, st>>>(a); };
+  if (vec == 8) {
+    if constexpr (sizeof(T) == 2) launch(rotary_kernel<T, 8, APPEND>);
+  } else if (vec == 4) {
+    launch(rotary_kernel<T, 4, APPEND>);
+  } else if (vec == 2) {
+    launch(rotary_kernel<T, 2, APPEND>);
+  } else {
+    launch(rotary_kernel<T, 1, APPEND>);
   }
   const cudaError_t e = cudaGetLastError();
   if (e != cudaSuccess)
