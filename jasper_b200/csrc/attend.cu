@@ -137,7 +137,7 @@ struct AttendParams {
   uint32_t group, head_tiles;  // query heads of a key-value head, and tiles of 8 NT of them
   uint32_t workers;
   bool by_worker;              // what parts.spans goes by
-  bool clustered;              // a cluster of blocks per row's head
+  uint32_t cluster;            // blocks to a row's head; 0: equal parts
   bool tiled_pages;            // pages are whole tiles: a tile lies in one page
 };
 
@@ -247,7 +247,9 @@ struct Attend {
   static constexpr int kTileBytes = TK * L::kRowBytes;   // keys, then as much values
   static constexpr int kStageBytes = 2 * kTileBytes;
   static constexpr int kRingBytes = WARPS * STAGES * kStageBytes;
-  static constexpr int kSmem = kRingBytes + WARPS * STAGES * 4 + kMaxListed * 8 + (kMaxListed + 1) * 8 + 8;
+  static constexpr int shared_bytes() {
+    return kRingBytes + WARPS * STAGES * 4 + kMaxListed * 8 + (kMaxListed + 1) * 8 + 8;
+  }
   static constexpr int KS = DP / 16;                     // k steps of Q K, head tiles of 16 of P V
   static constexpr int kChunkLanes = DP <= 64 ? 8 : DP <= 128 ? 16 : 32;  // lanes a row of 16-byte chunks takes
   static constexpr int kRowsPerCopy = 32 / kChunkLanes;
@@ -650,15 +652,18 @@ __global__ void __launch_bounds__(WARPS * 32) attend_kernel(const __grid_constan
 }
 
 // The same for few rows of few tokens, where a call's latency is what counts:
-// a cluster of kCluster blocks takes one row's head, its warps every
-// kCluster * WARPS-th tile, and the blocks' results are joined through
-// distributed shared memory, with no second kernel and no scratch.
-constexpr int kCluster = 8;
-constexpr uint64_t kMostClusters = 15, kClusterTokens = 6000;
+// a cluster of 1, 2, 4 or 8 blocks takes one row's head, its warps a tile each
+// in turn, and the blocks' results are joined through distributed shared
+// memory, with no second kernel and no scratch.
+constexpr int kCluster = 8;                // the largest
+constexpr uint64_t kTokensOfBlock = 1500;  // of heads of 128, at most
+// Fewer warps start, and are joined, sooner: 1000 tokens of 8 heads of 128
+// took 6.4 us with 8 warps a block, 7.2 with 12, 6.7 with 4; 4000 tokens 9.4,
+// 10.0 and 11.9.
+constexpr Ring cluster_ring_of(int DP) { return DP == 256 ? Ring{6, 2} : Ring{8, 3}; }
 
 template <typename T, int DP, int NT, int WARPS, int STAGES>
-__global__ void __cluster_dims__(kCluster, 1, 1) __launch_bounds__(WARPS * 32)
-attend_cluster_kernel(const __grid_constant__ AttendParams p) {
+__global__ void __launch_bounds__(WARPS * 32) attend_cluster_kernel(const __grid_constant__ AttendParams p) {
   using A = Attend<T, DP, NT, WARPS, STAGES>;
   constexpr int C = A::kColumns;
   extern __shared__ __align__(1024) unsigned char smem[];
@@ -678,7 +683,7 @@ attend_cluster_kernel(const __grid_constant__ AttendParams p) {
   const uint32_t rank = blockIdx.x;  // the grid is one cluster wide
   c.t = tiles_of(p.a, c.i);
   const int count = max(c.t.end - c.t.begin, 0);
-  const int first = int(rank) * WARPS + wid, step = kCluster * WARPS;
+  const int blocks = int(gridDim.x), first = int(rank) * WARPS + wid, step = blocks * WARPS;
   unsigned char* ring = smem + wid * STAGES * A::kStageBytes;
   if (p.a.c.head_dim < DP) {  // columns that no copy writes
     for (int i = lane; i < STAGES * A::kStageBytes / 16; i += 32)
@@ -755,13 +760,16 @@ attend_cluster_kernel(const __grid_constant__ AttendParams p) {
     return a;
   };
   const int dim = int(p.a.c.head_dim);
-  for (int e = int(rank) * WARPS * 32 + threadIdx.x; e < columns * DP; e += kCluster * WARPS * 32) {
+  for (int e = int(rank) * WARPS * 32 + threadIdx.x; e < columns * DP; e += step * 32) {
     const int column = e / DP, d = e % DP;
     float2 rl[kCluster];
     float part[kCluster];
     float ref = -INFINITY;
 #pragma unroll
     for (int b = 0; b < kCluster; b++) {
+      rl[b] = make_float2(-INFINITY, 0.0f);
+      part[b] = 0.0f;
+      if (b >= blocks) continue;
       asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];"
                    : "=f"(rl[b].x), "=f"(rl[b].y) : "r"(remote(&block_rl[column], b)) : "memory");
       asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(part[b]) : "r"(remote(&block_o[column][d], b)) : "memory");
@@ -900,7 +908,7 @@ struct Shape {
   int dp, nt, warps;
   uint32_t group, head_tiles, workers;
   uint64_t row_heads;
-  bool clustered;
+  uint32_t cluster;
 };
 Shape shape_of(const AttendArgs& a) {
   Shape s;
@@ -912,13 +920,17 @@ Shape shape_of(const AttendArgs& a) {
   s.warps = ring_of(s.dp, s.nt).warps;
   s.workers = uint32_t(sm_count() * s.warps);
   s.row_heads = uint64_t(a.n) * a.c.n_kv_heads * s.head_tiles;
-  // Few enough clusters that all run at once (15 of 8 do here, 16 do not: 7.5
-  // and 13 us), and rows short enough, by the table's width or the window,
-  // that the SMs they leave idle matter less than the second kernel.  One row,
-  // 8 heads of 128, clusters / equal parts: 7.2 / 10.0 us with 1000 tokens,
-  // 10.2 / 12.0 with 4000, 14.5 / 13.8 with 8000.
-  const uint64_t longest = uint64_t(a.c.max_pages) * a.c.page_size;
-  s.clustered = s.row_heads <= kMostClusters && (a.window && a.window < longest ? a.window : longest) <= kClusterTokens;
+  // Clusters as large as all run at once (15 of 8 blocks take 7 us, 16 take
+  // 13; 33 and 36 of 4, 7.8 and 13.4), where rows are short enough, by the
+  // table's width or the window, that unequal lengths cost less than the
+  // second kernel.  Clusters / equal parts, heads of 128: one row of 1000
+  // tokens and 8 heads 6.4 / 10.0 us, of 8000 14.0 / 14.0; 32 rows' heads of
+  // 4000 tokens 18 / 21, of 1000 to 4000 14 / 15; 64 of 4000 28 / 31, of 1000
+  // to 4000 26 / 24.
+  const uint64_t wide = uint64_t(a.c.max_pages) * a.c.page_size;
+  const uint64_t longest = a.window && a.window < wide ? a.window : wide;
+  s.cluster = s.row_heads <= 15 ? 8 : s.row_heads <= 32 ? 4 : s.row_heads <= 74 ? 2 : s.row_heads <= 148 ? 1 : 0;
+  if (longest * s.dp > kTokensOfBlock * 128 * s.cluster) s.cluster = 0;
   return s;
 }
 
@@ -944,19 +956,31 @@ void launch_typed(const AttendParams& p, cudaStream_t st) {
   static std::mutex m;
   static uint64_t ready = 0, cluster_ready = 0;  // devices where the kernels have their shared memory
   const uint64_t row_heads = uint64_t(p.a.n) * p.a.c.n_kv_heads * p.head_tiles;
-  if (p.clustered) {
-    auto cluster_kernel = attend_cluster_kernel<T, DP, NT, kWarps, kStages>;
-    allow_shared(cluster_kernel, A::kRingBytes, cluster_ready, m);
-    cluster_kernel<<<dim3(kCluster, uint32_t(row_heads)), A::kThreads, A::kRingBytes, st>>>(p);
-    check_cuda(cudaGetLastError(), "attend launch");
+  if (p.cluster) {
+    constexpr Ring ring = cluster_ring_of(DP);
+    using C = Attend<T, DP, NT, ring.warps, ring.stages>;
+    auto cluster_kernel = attend_cluster_kernel<T, DP, NT, ring.warps, ring.stages>;
+    allow_shared(cluster_kernel, C::kRingBytes, cluster_ready, m);
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3(p.cluster, uint32_t(row_heads));
+    cfg.blockDim = dim3(C::kThreads);
+    cfg.dynamicSmemBytes = C::kRingBytes;
+    cfg.stream = st;
+    cudaLaunchAttribute attr{};
+    attr.id = cudaLaunchAttributeClusterDimension;
+    attr.val.clusterDim.x = p.cluster;
+    attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
+    cfg.attrs = &attr;
+    cfg.numAttrs = 1;
+    check_cuda(cudaLaunchKernelEx(&cfg, cluster_kernel, p), "attend launch");
     return;
   }
-  allow_shared(kernel, A::kSmem, ready, m);
+  allow_shared(kernel, A::shared_bytes(), ready, m);
   if (p.parts.prefix) {
     prefix_kernel<<<1, 1024, 0, st>>>(p.a, p.parts.prefix);
     check_cuda(cudaGetLastError(), "attend prefix launch");
   }
-  kernel<<<p.workers / kWarps, A::kThreads, A::kSmem, st>>>(p);
+  kernel<<<p.workers / kWarps, A::kThreads, A::shared_bytes(), st>>>(p);
   check_cuda(cudaGetLastError(), "attend launch");
   // rows of one tile are never split
   if (uint64_t(p.a.c.max_pages) * p.a.c.page_size <= TK) return;
@@ -998,7 +1022,7 @@ void launch_any(const AttendParams& p, int dp, int nt, cudaStream_t st) {
 size_t attend_scratch_bytes(const AttendArgs& a) {
   if (a.n == 0 || a.n_q_heads == 0) return 0;
   const Shape s = shape_of(a);
-  if (s.clustered) return 0;
+  if (s.cluster) return 0;
   const size_t slots = size_t(2) * s.workers * 8 * s.nt;
   return aligned(slots * s.dp * sizeof(float)) + aligned(slots * sizeof(float2)) +
          aligned(s.workers * sizeof(int4)) + (a.n > uint32_t(kMaxListed) ? (size_t(a.n) + 1) * sizeof(int64_t) : 0);
@@ -1015,7 +1039,7 @@ void launch_attend(const AttendArgs& a, void* scratch, cudaStream_t st) {
   if (double(s.row_heads) * double(a.c.max_pages) * a.c.page_size > 4e18)
     throw std::invalid_argument("rows, heads and tokens are too many for one call");
   p.by_worker = s.row_heads > s.workers;
-  p.clustered = s.clustered;
+  p.cluster = s.cluster;
   p.tiled_pages = a.c.page_size % TK == 0;
   const size_t slots = size_t(2) * s.workers * 8 * s.nt;
   unsigned char* at = static_cast<unsigned char*>(scratch);
