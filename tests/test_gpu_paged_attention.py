@@ -109,6 +109,44 @@ def test_long_and_ragged_rows(cuda, lengths):
     check(c, q, out, lse)
 
 
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("dim", [40, 64, 80, 128, 256])
+@pytest.mark.parametrize("group,page_size", [(1, 16), (4, 7), (16, 16), (19, 24)])
+def test_rows_in_several_parts(cuda, dtype, dim, group, page_size):
+    """Long enough that a row's head is shared out, with its neighbours' ends
+    in the same parts."""
+    lengths = [13_000, 5, 0, 2900, 17]
+    c = make(lengths, kv_heads=1, dim=dim, dtype=dtype, page_size=page_size, layout="head" if group == 4 else "token")
+    q = queries(len(lengths), group, dim, dtype)
+    g = torch.Generator().manual_seed(3)
+    mask = torch.rand(len(lengths), 13_000, generator=g) < 0.7
+    mask[0, 4000:6000] = False                       # whole parts with nothing to attend to
+    out, lse = c.attend(0, q, mask=mask.cuda(), return_lse=True)
+    check(c, q, out, lse, mask=mask)
+    out, lse = c.attend(0, q, window=3001, return_lse=True)
+    check(c, q, out, lse, window=3001)
+
+
+def test_more_rows_and_heads_than_workers(cuda):
+    """2800 rows' heads, one row much longer than the others."""
+    lengths = [20 + (37 * i) % 90 for i in range(700)]
+    lengths[333], lengths[334], lengths[699] = 9000, 0, 1500
+    c = make(lengths, kv_heads=4, dim=64, page_size=16)
+    q = queries(len(lengths), 8, 64, torch.float16)
+    out, lse = c.attend(0, q, return_lse=True)
+    check(c, q, out, lse)
+
+
+@pytest.mark.parametrize("rows", [1, 8, 9, 16, 17, 37, 38, 74, 75])
+def test_few_rows_in_clusters(cuda, rows):
+    lengths = [(61 * i) % 180 for i in range(rows)]
+    lengths[-1] = 900
+    c = make(lengths, kv_heads=2, dim=64, dtype=torch.bfloat16)
+    q = queries(rows, 6, 64, torch.bfloat16)
+    out, lse = c.attend(0, q, return_lse=True)
+    check(c, q, out, lse)
+
+
 def test_many_short_rows(cuda):
     lengths = [(7 * i) % 50 for i in range(1100)]
     c = make(lengths, kv_heads=1, dim=8, page_size=8)
