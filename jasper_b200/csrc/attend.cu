@@ -834,17 +834,17 @@ __global__ void __launch_bounds__(join_warps(SHARED) * 32) join_kernel(const __g
     }
 #pragma unroll
     for (int b = 0; b < B; b++) {
-      if (j0 + SHARED * b >= span.z) rl[b].x = -INFINITY;  // read twice: counts once
+      if (j0 + SHARED * b >= span.z) rl[b].x = -INFINITY;  // read twice: weighs once
       top = fmaxf(top, rl[b].x);
     }
-    if (top == -INFINITY) continue;
-    const float keep = exp2_fast(ref - top);
+    const float r = top == -INFINITY ? 0.0f : top;  // parts without a score weigh nothing, unless they are NaN
+    const float keep = exp2_fast(ref - r);
     l *= keep;
 #pragma unroll
     for (int k = 0; k < N; k++) o[k] *= keep;
 #pragma unroll
     for (int b = 0; b < B; b++) {
-      const float f = exp2_fast(rl[b].x - top);
+      const float f = exp2_fast(rl[b].x - r);
       l += rl[b].y * f;
 #pragma unroll
       for (int k = 0; k < N; k++) o[k] += part[b][k] * f;

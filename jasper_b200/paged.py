@@ -14,11 +14,12 @@ there.
   new token of each row.
 
 Tensors are checked and passed on by a small CPython module
-(csrc/paged_torch.cc); the kernels are those of libjasper_b200.so (``jb_rotary``, ``jb_kv_append``,
-``jb_pages_*``, ``jb_paged_attention`` in include/jasper_b200.h).  Calls are
-asynchronous on torch's current stream of the cache's device and read nothing
-back: a row or page that does not fit sets a bit of the cache's status word,
-which :meth:`PagedCache.check` reads.  No reference counterpart.
+(csrc/paged_torch.cc); the kernels are those of libjasper_b200.so
+(``jb_rotary``, ``jb_kv_append``, ``jb_pages_*``, ``jb_paged_attention`` in
+include/jasper_b200.h).  Calls are asynchronous on torch's current stream of
+the cache's device and read nothing back: a row or page that does not fit sets
+a bit of the cache's status word, which :meth:`PagedCache.check` reads.  After
+a first call they can be captured into CUDA graphs.  No reference counterpart.
 """
 from __future__ import annotations
 
@@ -71,6 +72,8 @@ class Rotary:
             raise ValueError(f"layout must be 'half' or 'interleaved', got {layout!r}")
         if scaling not in (None, "linear", "ntk", "yarn"):
             raise ValueError(f"scaling must be None, 'linear', 'ntk' or 'yarn', got {scaling!r}")
+        if not base > 1:
+            raise ValueError(f"base must be above 1, got {base}")
         if scaling is not None and not factor > 0:
             raise ValueError(f"factor must be positive, got {factor}")
         if scaling == "ntk" and rot_dim <= 2:
@@ -161,6 +164,8 @@ class PagedCache:
             raise ValueError(f"refs must be a contiguous [{n_pages}]")
         if status is None:
             status = torch.zeros(1, dtype=torch.int32, device=device)
+        elif status.numel() != 1:
+            raise ValueError(f"status must have one element, got {status.numel()}")
         for t, name in ((table, "table"), (lengths, "lengths"), (refs, "refs"), (status, "status")):
             if t.dtype != torch.int32:
                 raise ValueError(f"{name} must be int32, got {t.dtype}")
@@ -259,8 +264,8 @@ class PagedCache:
         return self._native.attend(self._ref, layer, q, rows, scale, window, mask, return_lse, out)
 
     def check(self) -> None:
-        """Waits for the cache's stream, and raises what the calls since the
-        last check() could not do."""
+        """Waits for the current stream, and raises what the calls on it since
+        the last check() could not do."""
         bits = int(self.status.item())
         if bits:
             self.status.zero_()

@@ -190,6 +190,31 @@ def test_masked_tokens_may_hold_anything(cuda, value):
     assert all(torch.equal(out[0], out[i]) for i in range(4))
 
 
+@pytest.mark.parametrize("lengths", [[40], [900], [20_000, 3]])
+def test_nan_is_not_hidden(cuda, lengths):
+    """NaN in a query, or in a key or value that is attended to, comes out; in
+    the other heads and rows it does not."""
+    c = make(lengths, kv_heads=2, dim=64, poison=False)
+    q = queries(len(lengths), 4, 64, torch.float16)
+    clean, clean_lse = c.attend(0, q, return_lse=True)
+    bad = q.clone()
+    bad[0, 1, 5] = math.nan
+    out, lse = c.attend(0, bad, return_lse=True)
+    assert out[0, 1].isnan().all() and lse[0, 1].isnan()
+    keep = torch.ones_like(lse, dtype=torch.bool)
+    keep[0, 1] = False
+    assert torch.equal(out[keep], clean[keep]) and torch.equal(lse[keep], clean_lse[keep])
+    page = c.table[0, (lengths[0] - 1) // 16].long()
+    c.v[0, page, (lengths[0] - 1) % 16, 1, 7] = math.nan
+    out, lse = c.attend(0, q, return_lse=True)
+    assert out[0, 2:, 7].isnan().all() and torch.equal(lse, clean_lse)
+    out[0, 2:, 7] = clean[0, 2:, 7]
+    assert torch.equal(out, clean)
+    c.k[0, page, (lengths[0] - 1) % 16, 0, 3] = math.inf
+    out, lse = c.attend(0, q.abs(), return_lse=True)
+    assert out[0, :2].isnan().all() and lse[0, :2].isnan().all()
+
+
 def test_pages_that_are_not_there(cuda):
     c = make([100, 64, 48, 200], dim=64)
     c.table[0, 2] = -1

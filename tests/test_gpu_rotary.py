@@ -186,6 +186,8 @@ def test_refusals(cuda):
             r.apply(*bad)
     with pytest.raises(ValueError):
         r.apply(x, p, out=x.half())
+    with pytest.raises(ValueError, match="positions"):
+        r.apply(x[None], p[:2])
     c = make_cache([5], 4, 2, 16, torch.float16)
     k = torch.zeros(1, 2, 16, dtype=torch.float16, device="cuda")
     rows = torch.zeros(1, dtype=torch.int32, device="cuda")

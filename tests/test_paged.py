@@ -34,7 +34,8 @@ def test_scaled_frequencies():
 
 @pytest.mark.parametrize("kw", [{"rot_dim": 3}, {"rot_dim": 0}, {"rot_dim": 66}, {"layout": "pairs"},
                                 {"scaling": "other"}, {"scaling": "linear", "factor": 0.0},
-                                {"scaling": "ntk", "factor": 2.0, "rot_dim": 2}, {"scaling": "yarn", "factor": 2.0}])
+                                {"scaling": "ntk", "factor": 2.0, "rot_dim": 2}, {"scaling": "yarn", "factor": 2.0},
+                                {"base": 1.0}, {"base": -3.0}])
 def test_rotary_refusals(kw):
     with pytest.raises(ValueError):
         paged.Rotary(64, device="cpu", **kw)
