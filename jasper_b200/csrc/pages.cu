@@ -483,9 +483,10 @@ compact_plan_kernel(const jb_page_cache c, int32_t* remap, int32_t* moves) {
 
 // ── copies ───────────────────────────────────────────────────────────────
 // Pages src[i] -> dst[i] in keys, values and every layer, tokens[i] tokens of
-// each (null: all); n pairs, or *n_device.  HBM bounds it: a warp takes 4 KB
-// of one page of one plane at a time, eight 16-byte reads of each lane before
-// the first write.  On the way, with `remap` the rows' table is rewritten, and
+// each (null: all); n pairs, or *n_device.  HBM bounds it: a warp takes some 4
+// KB pieces of one page of one plane, eight 16-byte reads of each lane before
+// the first write (301 pages of 1 MB: 101 us, 6.3 TB/s; with four reads and
+// more warps 106).  On the way, with `remap` the rows' table is rewritten, and
 // with `parents` the whole pages of forked rows are shared.
 constexpr int kCopyThreads = 256, kCopyDepth = 8;
 
@@ -499,9 +500,10 @@ struct CopyArgs {
   // a page's tokens lie as runs: `flat`, all in one run; `by_head`, a run for
   // each head; else a run for each token and head
   bool flat, by_head;
+  uint32_t run;  // pieces of a plane's page that a warp takes one after the other
 };
 
-__global__ void __launch_bounds__(kCopyThreads) copy_pages_kernel(const __grid_constant__ CopyArgs a) {
+__global__ void __launch_bounds__(kCopyThreads, 3) copy_pages_kernel(const __grid_constant__ CopyArgs a) {
   const jb_page_cache& c = a.c;
   if (a.remap) {
     const uint64_t total = uint64_t(c.n_rows) * c.max_pages;
@@ -531,42 +533,43 @@ __global__ void __launch_bounds__(kCopyThreads) copy_pages_kernel(const __grid_c
   const uint32_t pairs = a.n_device ? uint32_t(max(*a.n_device, 0)) : a.n;
   const uint32_t planes = 2 * c.n_layers, row = c.head_dim / 8;  // 16-byte vectors of a head
   const uint32_t full = c.page_size * c.n_kv_heads * row;
-  const uint32_t pieces = (full + 32 * kCopyDepth - 1) / (32 * kCopyDepth);
-  const uint64_t units = uint64_t(pairs) * planes * pieces;
+  const uint32_t run = a.run * 32 * kCopyDepth, runs = (full + run - 1) / run;
+  const uint64_t units = uint64_t(pairs) * planes * runs;
   for (uint64_t unit = warp; unit < units; unit += step) {
-    const uint64_t item = unit / pieces;
-    const uint32_t piece = uint32_t(unit - item * pieces);
+    const uint64_t item = unit / runs;
     const uint32_t i = uint32_t(item / planes), plane = uint32_t(item - uint64_t(i) * planes);
+    const uint32_t begin = uint32_t(unit - item * runs) * run;
     const int32_t from = a.src[i], to = a.dst[i];
+    const uint32_t nt = a.tokens ? uint32_t(a.tokens[i]) : c.page_size;
     if (!page_ok(c, from) || !page_ok(c, to)) {
       if (lane == 0 && !a.tokens) atomicOr(c.status, kPagesBadToken);
       continue;
     }
-    const uint32_t nt = a.tokens ? uint32_t(a.tokens[i]) : c.page_size;
-    const uint32_t count = nt * c.n_kv_heads * row;
-    const uint32_t v0 = piece * 32 * kCopyDepth + lane;
+    const uint32_t count = min(nt * c.n_kv_heads * row, begin + run);
     uint16_t* base = static_cast<uint16_t*>(plane & 1 ? c.v : c.k) + int64_t(plane >> 1) * c.layer_stride;
     const uint16_t* s = base + from * c.page_stride;
     uint16_t* d = base + to * c.page_stride;
-    uint4 v[kCopyDepth];
-    int64_t off[kCopyDepth];
+    for (uint32_t v0 = begin + lane; v0 < count; v0 += 32 * kCopyDepth) {
+      uint4 v[kCopyDepth];
+      int64_t off[kCopyDepth];
 #pragma unroll
-    for (int k = 0; k < kCopyDepth; k++) {
-      const uint32_t u = v0 + 32 * k;
-      if (a.flat) {
-        off[k] = int64_t(u) * 8;
-      } else if (a.by_head) {
-        const uint32_t h = u / (nt * row);
-        off[k] = int64_t(h) * c.head_stride + int64_t(u - h * nt * row) * 8;
-      } else {
-        const uint32_t th = u / row, t = th / c.n_kv_heads;
-        off[k] = int64_t(t) * c.token_stride + int64_t(th - t * c.n_kv_heads) * c.head_stride + int64_t(u - th * row) * 8;
+      for (int k = 0; k < kCopyDepth; k++) {
+        const uint32_t u = v0 + 32 * k;
+        if (a.flat) {
+          off[k] = int64_t(u) * 8;
+        } else if (a.by_head) {
+          const uint32_t h = u / (nt * row);
+          off[k] = int64_t(h) * c.head_stride + int64_t(u - h * nt * row) * 8;
+        } else {
+          const uint32_t th = u / row, t = th / c.n_kv_heads;
+          off[k] = int64_t(t) * c.token_stride + int64_t(th - t * c.n_kv_heads) * c.head_stride + int64_t(u - th * row) * 8;
+        }
+        if (u < count) v[k] = *reinterpret_cast<const uint4*>(s + off[k]);
       }
-      if (u < count) v[k] = *reinterpret_cast<const uint4*>(s + off[k]);
-    }
 #pragma unroll
-    for (int k = 0; k < kCopyDepth; k++)
-      if (v0 + 32 * k < count) *reinterpret_cast<uint4*>(d + off[k]) = v[k];
+      for (int k = 0; k < kCopyDepth; k++)
+        if (v0 + 32 * k < count) *reinterpret_cast<uint4*>(d + off[k]) = v[k];
+    }
   }
 }
 
@@ -578,9 +581,13 @@ void launch_copies(CopyArgs a, cudaStream_t st) {
   a.flat = token_rows || (a.by_head && a.tokens == nullptr && c.head_stride == ps * dim);
   const uint64_t full = uint64_t(c.page_size) * c.n_kv_heads * (c.head_dim / 8);
   if (full > 0x7FFFFFFFull) throw std::invalid_argument("a page is too large");
-  const uint64_t units = uint64_t(a.n) * 2 * c.n_layers * ((full + 32 * kCopyDepth - 1) / (32 * kCopyDepth));
-  const uint64_t blocks = (units + kCopyThreads / 32 - 1) / (kCopyThreads / 32);
   constexpr uint64_t kMost = 148 * 8;
+  const uint64_t pieces = (full + 32 * kCopyDepth - 1) / (32 * kCopyDepth);
+  uint64_t units = uint64_t(a.n) * 2 * c.n_layers * pieces;
+  a.run = uint32_t(units / (kMost * (kCopyThreads / 32) * 2));  // two units at least for every warp
+  a.run = a.run < 1 ? 1 : a.run > pieces ? uint32_t(pieces) : a.run;
+  units = uint64_t(a.n) * 2 * c.n_layers * ((pieces + a.run - 1) / a.run);
+  const uint64_t blocks = (units + kCopyThreads / 32 - 1) / (kCopyThreads / 32);
   copy_pages_kernel<<<uint32_t(blocks < kMost ? (blocks ? blocks : 1) : kMost), kCopyThreads, 0, st>>>(a);
   check_launch("copy pages");
 }
