@@ -75,14 +75,15 @@ def _build_paged_module(verbose: bool) -> Path:
     import sysconfig
 
     import torch
-    from torch.utils.cpp_extension import include_paths
     src = CSRC / "paged_torch.cc"
     out = LIB / "jasper_paged_torch.so"
     if out.exists() and out.stat().st_mtime > max(src.stat().st_mtime, _headers_mtime()):
         return out
-    torch_lib = Path(torch.__file__).resolve().parent / "lib"
+    torch_dir = Path(torch.__file__).resolve().parent
+    torch_lib = torch_dir / "lib"
     cmd = ["g++", "-std=c++17", "-O2", "-fPIC", "-shared", "-fvisibility=hidden", "-o", str(out), str(src),
-           f"-I{sysconfig.get_paths()['include']}", *(f"-I{p}" for p in include_paths()),
+           f"-I{sysconfig.get_paths()['include']}", f"-I{torch_dir / 'include'}",
+           f"-I{torch_dir / 'include' / 'torch' / 'csrc' / 'api' / 'include'}",
            "-I/usr/local/cuda/include", f"-D_GLIBCXX_USE_CXX11_ABI={int(torch.compiled_with_cxx11_abi())}",
            f"-L{torch_lib}", "-ltorch_python", "-ltorch", "-ltorch_cpu", "-ltorch_cuda", "-lc10",
            "-lc10_cuda", f"-Wl,-rpath,{torch_lib}"]
