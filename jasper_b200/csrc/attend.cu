@@ -183,6 +183,7 @@ __device__ __forceinline__ int64_t block_sum_scan(int64_t v, int64_t* total) {
 
 // The tiles before each query, for more queries than a block keeps itself.
 __global__ void __launch_bounds__(1024) prefix_kernel(const AttendArgs a, int64_t* prefix) {
+  follow();
   int64_t done = 0;
   for (uint64_t base = 0; base < a.n; base += 1024) {
     const uint64_t i = base + threadIdx.x;
@@ -606,7 +607,7 @@ __global__ void __launch_bounds__(WARPS * 32) attend_kernel(const __grid_constan
   typename A::Lists lists{row, len, prefix};
   const int wid = threadIdx.x >> 5;
   A self{p, lists, int(threadIdx.x & 31)};
-  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  follow();
   if (p.a.c.head_dim < DP)  // columns that no copy writes
     for (int i = threadIdx.x; i < A::kRingBytes / 16; i += A::kThreads)
       reinterpret_cast<uint4*>(smem)[i] = make_uint4(0, 0, 0, 0);
@@ -671,6 +672,7 @@ __global__ void __launch_bounds__(WARPS * 32) attend_cluster_kernel(const __grid
   __shared__ float2 warp_rl[WARPS][C];   // a warp's references and sums
   __shared__ float2 block_rl[C];
   __shared__ float block_o[C][DP];
+  follow();
   const int wid = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const typename A::Lists none{nullptr, nullptr, nullptr};
   const A self{p, none, lane};
@@ -810,7 +812,7 @@ __global__ void __launch_bounds__(join_warps(SHARED) * 32) join_kernel(const __g
   __shared__ float2 share_rl[SHARED];
   const int lane = threadIdx.x & 31, wid = threadIdx.x >> 5;
   const uint32_t item = SHARED == 1 ? blockIdx.x * kJoinSpans + wid : blockIdx.x;
-  asm volatile("griddepcontrol.wait;" ::: "memory");
+  follow();
   if (item >= spans) return;
   const int4 span = p.parts.spans[item];
   const int column = blockIdx.y;
@@ -961,45 +963,25 @@ void launch_typed(const AttendParams& p, cudaStream_t st) {
     using C = Attend<T, DP, NT, ring.warps, ring.stages>;
     auto cluster_kernel = attend_cluster_kernel<T, DP, NT, ring.warps, ring.stages>;
     allow_shared(cluster_kernel, C::kRingBytes, cluster_ready, m);
-    cudaLaunchConfig_t cfg{};
-    cfg.gridDim = dim3(p.cluster, uint32_t(row_heads));
-    cfg.blockDim = dim3(C::kThreads);
-    cfg.dynamicSmemBytes = C::kRingBytes;
-    cfg.stream = st;
-    cudaLaunchAttribute attr{};
-    attr.id = cudaLaunchAttributeClusterDimension;
-    attr.val.clusterDim.x = p.cluster;
-    attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
-    cfg.attrs = &attr;
-    cfg.numAttrs = 1;
-    check_cuda(cudaLaunchKernelEx(&cfg, cluster_kernel, p), "attend launch");
+    launch("attend", cluster_kernel, dim3(p.cluster, uint32_t(row_heads)), C::kThreads, C::kRingBytes, st, p.cluster, p);
     return;
   }
   allow_shared(kernel, A::shared_bytes(), ready, m);
   if (p.parts.prefix) {
-    prefix_kernel<<<1, 1024, 0, st>>>(p.a, p.parts.prefix);
-    check_cuda(cudaGetLastError(), "attend prefix launch");
+    launch("attend prefix", prefix_kernel, dim3(1), 1024, 0, st, 0, p.a, p.parts.prefix);
   }
-  kernel<<<p.workers / kWarps, A::kThreads, A::shared_bytes(), st>>>(p);
-  check_cuda(cudaGetLastError(), "attend launch");
+  launch("attend", kernel, dim3(p.workers / kWarps), A::kThreads, A::shared_bytes(), st, 0, p);
   // rows of one tile are never split
   if (uint64_t(p.a.c.max_pages) * p.a.c.page_size <= TK) return;
   const uint32_t spans = p.by_worker ? p.workers : uint32_t(row_heads);
   const uint32_t parts = p.workers / spans;  // about as many to a span
   const int shared = parts >= 48 ? 16 : parts >= 6 ? 4 : 1;
-  cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3(shared == 1 ? (spans + kJoinSpans - 1) / kJoinSpans : spans, p.group < 8 * NT ? p.group : 8 * NT);
-  cfg.blockDim = dim3(join_warps(shared) * 32);
-  cfg.stream = st;
-  cudaLaunchAttribute attr{};
-  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr.val.programmaticStreamSerializationAllowed = 1;
-  cfg.attrs = &attr;
-  cfg.numAttrs = 1;
   auto join = shared == 16  ? join_kernel<T, DP, NT, 16>
               : shared == 4 ? join_kernel<T, DP, NT, 4>
                             : join_kernel<T, DP, NT, 1>;
-  check_cuda(cudaLaunchKernelEx(&cfg, join, p, spans), "attend join launch");
+  launch("attend join", join,
+         dim3(shared == 1 ? (spans + kJoinSpans - 1) / kJoinSpans : spans, p.group < 8 * NT ? p.group : 8 * NT),
+         join_warps(shared) * 32, 0, st, 0, p, spans);
 }
 
 template <typename T>

@@ -7,9 +7,48 @@
 #include <cuda_runtime.h>
 #include <cstddef>
 #include <cstdint>
+#include <stdexcept>
+#include <string>
 #include "../../include/jasper_b200.h"
 
 namespace jb {
+
+// A decode step is a chain of kernels of a few microseconds, so each is launched
+// while the one before it still runs (programmatic dependent launch), and
+// begins with follow(): it lets the next one start, and waits until all that
+// came before has ended and can be read.  Every thread of every kernel here
+// calls it before it touches global memory or returns, so that no kernel ends
+// before its predecessors.  In a stream, 8 heads of one row of 1000 tokens: 8.2
+// -> 6.5 us a call; rotary positions of 4099 x 12 x 80 float32: 8.2 -> 6.3.
+__device__ __forceinline__ void follow() {
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+}
+
+// Launches a kernel that begins with follow(); cluster > 0: in clusters of so
+// many blocks (a kernel's own cluster size otherwise).
+template <typename... P, typename... A>
+void launch(const char* what, void (*kernel)(P...), dim3 grid, uint32_t threads, size_t shared, cudaStream_t st,
+            uint32_t cluster, const A&... args) {
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3(threads);
+  cfg.dynamicSmemBytes = shared;
+  cfg.stream = st;
+  cudaLaunchAttribute attrs[2]{};
+  attrs[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attrs[0].val.programmaticStreamSerializationAllowed = 1;
+  attrs[1].id = cudaLaunchAttributeClusterDimension;
+  attrs[1].val.clusterDim.x = cluster;
+  attrs[1].val.clusterDim.y = attrs[1].val.clusterDim.z = 1;
+  cfg.attrs = attrs;
+  cfg.numAttrs = cluster ? 2 : 1;
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, args...);
+  if (e != cudaSuccess) {
+    cudaGetLastError();
+    throw std::runtime_error(std::string(what) + " launch: " + cudaGetErrorString(e));
+  }
+}
 
 // Bits of a cache's status word (jb_page_cache::status).
 constexpr int kPagesExhausted = JB_PAGES_EXHAUSTED;

@@ -19,12 +19,6 @@ constexpr uint32_t kRowsInBlock = 2048;  // rows of a call, and of the table, wh
 constexpr uint32_t kOwnersInBlock = 8192;  // a block keeps in its shared memory
 constexpr size_t kPlanShared = 4 * kRowsInBlock * 4 + kOwnersInBlock * 4 + kBlockPages * 2;
 
-void check_launch(const char* what) {
-  const cudaError_t e = cudaGetLastError();
-  if (e != cudaSuccess)
-    throw std::runtime_error(std::string(what) + " launch: " + cudaGetErrorString(e));
-}
-
 __device__ __forceinline__ bool row_ok(const jb_page_cache& c, int32_t r) {
   return r >= 0 && uint32_t(r) < c.n_rows;
 }
@@ -244,6 +238,7 @@ __global__ void __cluster_dims__(BLOCKS, 1, 1) __launch_bounds__(kPlanThreads)
 extend_kernel(const jb_page_cache c, const int32_t* rows, const int32_t* tokens, uint32_t n, int32_t* scratch) {
   extern __shared__ __align__(16) unsigned char shared[];
   __shared__ int box[BLOCKS];
+  follow();
   cluster_arrive<BLOCKS>();
   const PoolPart part(c, BLOCKS);
   const uint32_t bits = free_bits(c, part, part.first(0));
@@ -307,6 +302,7 @@ fork_kernel(const jb_page_cache c, const int32_t* parents, const int32_t* childr
             int32_t* scratch) {
   extern __shared__ __align__(16) unsigned char shared[];
   __shared__ int box[BLOCKS];
+  follow();
   cluster_arrive<BLOCKS>();
   const PoolPart part(c, BLOCKS);
   const uint32_t bits = free_bits(c, part, part.first(0));
@@ -371,7 +367,8 @@ fork_kernel(const jb_page_cache c, const int32_t* parents, const int32_t* childr
 }
 
 __global__ void __launch_bounds__(256)
-free_kernel(const jb_page_cache c, const int32_t* rows, uint32_t n) {
+free_kernel(const jb_page_cache c, const int32_t* rows) {
+  follow();
   const uint32_t i = blockIdx.x;
   const int32_t r = rows[i];
   if (!row_ok(c, r)) {
@@ -391,6 +388,7 @@ free_kernel(const jb_page_cache c, const int32_t* rows, uint32_t n) {
 // owner[row] = the first i that names the row
 __global__ void __launch_bounds__(kPlanThreads)
 adopt_claim_kernel(const jb_page_cache c, const int32_t* rows, uint32_t n, int32_t* owner) {
+  follow();
   for (uint32_t r = threadIdx.x; r < c.n_rows; r += blockDim.x) owner[r] = 0x7FFFFFFF;
   __syncthreads();
   for (uint32_t i = threadIdx.x; i < n; i += blockDim.x)
@@ -400,6 +398,7 @@ adopt_claim_kernel(const jb_page_cache c, const int32_t* rows, uint32_t n, int32
 __global__ void __launch_bounds__(128)
 adopt_kernel(const jb_page_cache c, const int32_t* rows, const int32_t* pages, int64_t pages_stride,
              uint32_t m, const int32_t* lengths, const int32_t* owner) {
+  follow();
   const uint32_t i = blockIdx.x;
   const int32_t r = rows[i];
   const int64_t ps = c.page_size;
@@ -428,6 +427,7 @@ template <int BLOCKS>
 __global__ void __cluster_dims__(BLOCKS, 1, 1) __launch_bounds__(kPlanThreads)
 compact_plan_kernel(const jb_page_cache c, int32_t* remap, int32_t* moves) {
   __shared__ int live_box[BLOCKS], hole_box[BLOCKS], mover_box[BLOCKS];
+  follow();
   cluster_arrive<BLOCKS>();
   const PoolPart part(c, BLOCKS);
   const uint32_t bits0 = free_bits(c, part, part.first(0));
@@ -505,6 +505,7 @@ struct CopyArgs {
 
 __global__ void __launch_bounds__(kCopyThreads, 3) copy_pages_kernel(const __grid_constant__ CopyArgs a) {
   const jb_page_cache& c = a.c;
+  follow();
   if (a.remap) {
     const uint64_t total = uint64_t(c.n_rows) * c.max_pages;
     for (uint64_t i = uint64_t(blockIdx.x) * kCopyThreads + threadIdx.x; i < total; i += uint64_t(gridDim.x) * kCopyThreads) {
@@ -588,8 +589,8 @@ void launch_copies(CopyArgs a, cudaStream_t st) {
   a.run = a.run < 1 ? 1 : a.run > pieces ? uint32_t(pieces) : a.run;
   units = uint64_t(a.n) * 2 * c.n_layers * ((pieces + a.run - 1) / a.run);
   const uint64_t blocks = (units + kCopyThreads / 32 - 1) / (kCopyThreads / 32);
-  copy_pages_kernel<<<uint32_t(blocks < kMost ? (blocks ? blocks : 1) : kMost), kCopyThreads, 0, st>>>(a);
-  check_launch("copy pages");
+  launch("copy pages", copy_pages_kernel, dim3(uint32_t(blocks < kMost ? (blocks ? blocks : 1) : kMost)), kCopyThreads,
+         0, st, 0, a);
 }
 
 // Launches a plan kernel; its shared memory is allowed once per device.
@@ -598,17 +599,19 @@ void launch_plan_of(const char* what, cudaStream_t st, A... args) {
   static std::mutex m;
   static uint64_t ready = 0;
   int dev = 0;
-  if (cudaGetDevice(&dev) != cudaSuccess) check_launch(what);
+  cudaError_t e = cudaGetDevice(&dev);
   {
     std::lock_guard<std::mutex> lock(m);
-    if (!(ready >> dev & 1)) {
-      if (cudaFuncSetAttribute(Kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, int(kPlanShared)) != cudaSuccess)
-        check_launch(what);
-      ready |= uint64_t(1) << dev;
+    if (e == cudaSuccess && !(ready >> dev & 1)) {
+      e = cudaFuncSetAttribute(Kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, int(kPlanShared));
+      if (e == cudaSuccess) ready |= uint64_t(1) << dev;
     }
   }
-  Kernel<<<BLOCKS, kPlanThreads, kPlanShared, st>>>(args...);
-  check_launch(what);
+  if (e != cudaSuccess) {
+    cudaGetLastError();
+    throw std::runtime_error(std::string(what) + ": " + cudaGetErrorString(e));
+  }
+  launch(what, Kernel, dim3(BLOCKS), kPlanThreads, kPlanShared, st, 0, args...);
 }
 #define JB_LAUNCH_PLAN(kernel, what, c, ...)                                                    \
   do {                                                                                          \
@@ -647,18 +650,15 @@ void launch_fork(const jb_page_cache& c, const int32_t* parents, const int32_t* 
 
 void launch_free(const jb_page_cache& c, const int32_t* rows, uint32_t n, cudaStream_t st) {
   if (n == 0) return;
-  free_kernel<<<n, 256, 0, st>>>(c, rows, n);
-  check_launch("free");
+  launch("free", free_kernel, dim3(n), 256, 0, st, 0, c, rows);
 }
 
 void launch_adopt(const jb_page_cache& c, const int32_t* rows, const int32_t* pages,
                   int64_t pages_stride, uint32_t m, const int32_t* lengths, uint32_t n,
                   int32_t* scratch, cudaStream_t st) {
   if (n == 0) return;
-  adopt_claim_kernel<<<1, kPlanThreads, 0, st>>>(c, rows, n, scratch);
-  check_launch("adopt");
-  adopt_kernel<<<n, 128, 0, st>>>(c, rows, pages, pages_stride, m, lengths, scratch);
-  check_launch("adopt");
+  launch("adopt", adopt_claim_kernel, dim3(1), kPlanThreads, 0, st, 0, c, rows, n, scratch);
+  launch("adopt", adopt_kernel, dim3(n), 128, 0, st, 0, c, rows, pages, pages_stride, m, lengths, scratch);
 }
 
 void launch_compact(const jb_page_cache& c, int32_t* remap, int32_t* scratch, cudaStream_t st) {

@@ -70,6 +70,7 @@ __global__ void __launch_bounds__(kMaxThreads, kBlocks) rotary_kernel(const __gr
   extern __shared__ float2 cs[];  // [tokens][VEC][rot / 2 / VEC]: neighbouring threads read neighbours
   __shared__ int64_t place[kMaxTokens];
   using V = Vec<T, VEC>;
+  follow();
   const uint32_t half = a.r.rot / 2, pair_units = half / VEC;
   const uint64_t t0 = uint64_t(blockIdx.x) * a.tokens_per_block;
   const uint32_t nt = uint32_t(min(uint64_t(a.tokens_per_block), a.n_tokens - t0));
@@ -252,19 +253,16 @@ void launch_typed(RotaryParams a, cudaStream_t st) {
   const uint64_t blocks = (a.n_tokens + a.tokens_per_block - 1) / a.tokens_per_block;
   if (blocks > 0x7FFFFFFFull) throw std::invalid_argument("too many tokens");
   const size_t smem = size_t(a.tokens_per_block) * (a.r.rot / 2) * sizeof(float2);
-  auto launch = [&](auto kernel) { kernel<<<uint32_t(blocks), threads, smem, st>>>(a); };
+  const dim3 grid(static_cast<uint32_t>(blocks));
   if (vec == 8) {
-    if constexpr (sizeof(T) == 2) launch(rotary_kernel<T, 8, APPEND>);
+    if constexpr (sizeof(T) == 2) launch("rotary", rotary_kernel<T, 8, APPEND>, grid, threads, smem, st, 0, a);
   } else if (vec == 4) {
-    launch(rotary_kernel<T, 4, APPEND>);
+    launch("rotary", rotary_kernel<T, 4, APPEND>, grid, threads, smem, st, 0, a);
   } else if (vec == 2) {
-    launch(rotary_kernel<T, 2, APPEND>);
+    launch("rotary", rotary_kernel<T, 2, APPEND>, grid, threads, smem, st, 0, a);
   } else {
-    launch(rotary_kernel<T, 1, APPEND>);
+    launch("rotary", rotary_kernel<T, 1, APPEND>, grid, threads, smem, st, 0, a);
   }
-  const cudaError_t e = cudaGetLastError();
-  if (e != cudaSuccess)
-    throw std::runtime_error(std::string("rotary launch: ") + cudaGetErrorString(e));
 }
 
 template <bool APPEND>
