@@ -138,6 +138,9 @@ struct AttendParams {
   uint32_t workers;
   bool by_worker;              // what parts.spans goes by
   uint32_t cluster;            // blocks to a row's head; 0: equal parts
+  uint32_t share;              // with one block: rows' heads in it
+  uint32_t warps_each;         // a block's warps to a row's head
+  uint64_t row_heads;
   bool tiled_pages;            // pages are whole tiles: a tile lies in one page
 };
 
@@ -653,9 +656,10 @@ __global__ void __launch_bounds__(WARPS * 32) attend_kernel(const __grid_constan
 }
 
 // The same for few rows of few tokens, where a call's latency is what counts:
-// a cluster of 1, 2, 4 or 8 blocks takes one row's head, its warps a tile each
-// in turn, and the blocks' results are joined through distributed shared
-// memory, with no second kernel and no scratch.
+// a cluster of 1, 2, 4 or 8 blocks, or some of one block's warps, take one row's
+// head, a tile each in turn, and their results are joined through shared, and
+// the blocks' through distributed shared memory, with no second kernel and no
+// scratch.
 constexpr int kCluster = 8;                // the largest
 constexpr uint64_t kTokensOfBlock = 1500;  // of heads of 128, at most
 // Fewer warps start, and are joined, sooner: 1000 tokens of 8 heads of 128
@@ -669,23 +673,31 @@ __global__ void __launch_bounds__(WARPS * 32) attend_cluster_kernel(const __grid
   constexpr int C = A::kColumns;
   extern __shared__ __align__(1024) unsigned char smem[];
   __shared__ uint32_t valid[WARPS * STAGES];
-  __shared__ float2 warp_rl[WARPS][C];   // a warp's references and sums
-  __shared__ float2 block_rl[C];
-  __shared__ float block_o[C][DP];
+  constexpr int OS = DP + 4;              // floats from a column of a warp's result to the next: no bank conflicts
+  __shared__ float2 warp_rl[WARPS][C];    // a warp's references and sums
+  __shared__ float warp_f[WARPS][C];      // what its result weighs in its group's
+  __shared__ float2 group_rl[WARPS][C];
+  __shared__ __align__(16) float block_o[C][DP];
   follow();
   const int wid = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const typename A::Lists none{nullptr, nullptr, nullptr};
   const A self{p, none, lane};
-  const uint32_t heads = self.head_rows();
-  Cursor c;
-  c.i = blockIdx.y / heads;
-  c.vh = blockIdx.y % heads;
-  typename A::State s;
-  self.begin(s, c.i, c.vh);
+  // the warps of a row's head: `each` of a block's, in `blocks` blocks
+  const int each = int(p.warps_each), group = wid / each, blocks = int(gridDim.x);
   const uint32_t rank = blockIdx.x;  // the grid is one cluster wide
-  c.t = tiles_of(p.a, c.i);
+  const uint32_t item = blockIdx.y * (WARPS / each) + group;
+  const uint32_t heads = self.head_rows();
+  const bool has = item < p.row_heads;
+  Cursor c{};
+  typename A::State s;
+  if (has) {
+    c.i = item / heads;
+    c.vh = item % heads;
+    self.begin(s, c.i, c.vh);
+    c.t = tiles_of(p.a, c.i);
+  }
   const int count = max(c.t.end - c.t.begin, 0);
-  const int blocks = int(gridDim.x), first = int(rank) * WARPS + wid, step = blocks * WARPS;
+  const int first = int(rank) * each + wid % each, step = blocks * each;
   unsigned char* ring = smem + wid * STAGES * A::kStageBytes;
   if (p.a.c.head_dim < DP) {  // columns that no copy writes
     for (int i = lane; i < STAGES * A::kStageBytes / 16; i += 32)
@@ -696,11 +708,16 @@ __global__ void __launch_bounds__(WARPS * 32) attend_cluster_kernel(const __grid
     const uint32_t stage0 = smem_addr(ring);
     uint32_t* mask_of = valid + wid * STAGES;
     int to_load = first, load_stage = 0;
+    c.tile = c.t.begin + first;
+    typename A::Place place = self.place_of(c);
     auto load_next = [&] {
       if (to_load < count) {
-        c.tile = c.t.begin + to_load;
-        self.load_tile(stage0 + load_stage * A::kStageBytes, mask_of + load_stage, c, self.place_of(c));
+        self.load_tile(stage0 + load_stage * A::kStageBytes, mask_of + load_stage, c, place);
         to_load += step;
+        if (to_load < count) {  // the next one's page is looked up ahead
+          c.tile = c.t.begin + to_load;
+          place = self.place_of(c);
+        }
       }
       copies_commit();
       load_stage = load_stage + 1 == STAGES ? 0 : load_stage + 1;
@@ -719,6 +736,12 @@ __global__ void __launch_bounds__(WARPS * 32) attend_cluster_kernel(const __grid
     }
     copies_wait<0>();
     __syncwarp();
+  }
+  if (blocks == 1 && each == 1) {  // the warp has it all
+    if (has) self.finish(s, c.i, c.vh, -1);
+    return;
+  }
+  if (first < count) {
     // the ring is done with: it takes the warp's result
     float* o = reinterpret_cast<float*>(ring);
 #pragma unroll
@@ -732,65 +755,93 @@ __global__ void __launch_bounds__(WARPS * 32) attend_cluster_kernel(const __grid
         if (lane < 4) warp_rl[wid][column] = make_float2(s.ref[n][j], l);
 #pragma unroll
         for (int k = 0; k < A::KS; k++) {
-          o[column * DP + 16 * k + lane / 4] = s.o[n][k][j];
-          o[column * DP + 16 * k + lane / 4 + 8] = s.o[n][k][j + 2];
+          o[column * OS + 16 * k + lane / 4] = s.o[n][k][j];
+          o[column * OS + 16 * k + lane / 4 + 8] = s.o[n][k][j + 2];
         }
       }
   }
   __syncthreads();
-  const int warps = min(WARPS, max(0, count - int(rank) * WARPS));  // those that had tiles
-  const int columns = min(C, int(p.group - (c.vh % p.head_tiles) * C));
-  for (int e = threadIdx.x; e < columns * DP; e += WARPS * 32) {
-    const int column = e / DP, d = e % DP;
-    float ref = -INFINITY;
-    for (int w = 0; w < warps; w++) ref = fmaxf(ref, warp_rl[w][column].x);
+  const int warp0 = group * each, t = int(threadIdx.x) - warp0 * 32;
+  const int warps = min(each, max(0, count - int(rank) * each));  // those that had tiles
+  const int columns = has ? min(C, int(p.group - (c.vh % p.head_tiles) * C)) : 0;
+  if (t < each * C) {
+    const int w = t / C, column = t % C;
+    float ref = -INFINITY, l = 0.0f;
+    for (int i = 0; i < warps; i++) ref = fmaxf(ref, warp_rl[warp0 + i][column].x);
     const float r = ref == -INFINITY ? 0.0f : ref;
-    float o = 0.0f, l = 0.0f;
-    for (int w = 0; w < warps; w++) {
-      const float2 rl = warp_rl[w][column];
-      const float f = exp2_fast(rl.x - r);
-      o += reinterpret_cast<const float*>(smem + w * STAGES * A::kStageBytes)[e] * f;
-      l += rl.y * f;
+    if (w < warps) warp_f[warp0 + w][column] = exp2_fast(warp_rl[warp0 + w][column].x - r);
+    if (w == 0) {
+      for (int i = 0; i < warps; i++) l += warp_rl[warp0 + i][column].y * exp2_fast(warp_rl[warp0 + i][column].x - r);
+      group_rl[group][column] = make_float2(ref, l);
     }
-    block_o[column][d] = o;
-    if (d == 0) block_rl[column] = make_float2(ref, l);
   }
+  __syncthreads();
+  // four elements of a column at a time
+  const int dim = int(p.a.c.head_dim);
+  auto put = [&](int column, int d, float ref, float4 o, float l) {
+    const uint32_t h = self.head_of(c.vh, column);
+    const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+    if (d < dim) {
+      T* out = static_cast<T*>(p.a.out.p) + int64_t(c.i) * p.a.out.token_stride + int64_t(h) * p.a.out.head_stride + d;
+      alignas(8) T v[4] = {Mma<T>::from(o.x * inv), Mma<T>::from(o.y * inv), Mma<T>::from(o.z * inv),
+                           Mma<T>::from(o.w * inv)};
+      *reinterpret_cast<uint2*>(out) = *reinterpret_cast<const uint2*>(v);
+    }
+    if (d == 0 && p.a.lse)
+      p.a.lse[int64_t(c.i) * p.a.n_q_heads + h] = l == 0.0f ? -INFINITY : (ref + log2f(l)) * 0.6931471805599453f;
+  };
+  for (int e = 4 * t; e < columns * DP; e += 4 * each * 32) {
+    const int column = e / DP, d = e % DP;
+    float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    for (int w = warp0; w < warp0 + warps; w++) {
+      const float f = warp_f[w][column];
+      const float4 x = *reinterpret_cast<const float4*>(
+          reinterpret_cast<const float*>(smem + w * STAGES * A::kStageBytes) + column * OS + d);
+      o.x += x.x * f;
+      o.y += x.y * f;
+      o.z += x.z * f;
+      o.w += x.w * f;
+    }
+    if (blocks == 1) put(column, d, group_rl[group][column].x, o, group_rl[group][column].y);
+    else *reinterpret_cast<float4*>(&block_o[column][d]) = o;
+  }
+  if (blocks == 1) return;
   asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
   auto remote = [&](const void* at, int block) {
     uint32_t a;
     asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(smem_addr(at)), "r"(block));
     return a;
   };
-  const int dim = int(p.a.c.head_dim);
-  for (int e = int(rank) * WARPS * 32 + threadIdx.x; e < columns * DP; e += step * 32) {
+  for (int e = 4 * (int(rank) * WARPS * 32 + int(threadIdx.x)); e < columns * DP; e += 4 * step * 32) {
     const int column = e / DP, d = e % DP;
     float2 rl[kCluster];
-    float part[kCluster];
+    float4 part[kCluster];
     float ref = -INFINITY;
 #pragma unroll
     for (int b = 0; b < kCluster; b++) {
       rl[b] = make_float2(-INFINITY, 0.0f);
-      part[b] = 0.0f;
+      part[b] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
       if (b >= blocks) continue;
       asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];"
-                   : "=f"(rl[b].x), "=f"(rl[b].y) : "r"(remote(&block_rl[column], b)) : "memory");
-      asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(part[b]) : "r"(remote(&block_o[column][d], b)) : "memory");
+                   : "=f"(rl[b].x), "=f"(rl[b].y) : "r"(remote(&group_rl[0][column], b)) : "memory");
+      asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
+                   : "=f"(part[b].x), "=f"(part[b].y), "=f"(part[b].z), "=f"(part[b].w)
+                   : "r"(remote(&block_o[column][d], b)) : "memory");
       ref = fmaxf(ref, rl[b].x);
     }
     const float r = ref == -INFINITY ? 0.0f : ref;
-    float o = 0.0f, l = 0.0f;
+    float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    float l = 0.0f;
 #pragma unroll
     for (int b = 0; b < kCluster; b++) {
       const float f = exp2_fast(rl[b].x - r);
-      o += part[b] * f;
+      o.x += part[b].x * f;
+      o.y += part[b].y * f;
+      o.z += part[b].z * f;
+      o.w += part[b].w * f;
       l += rl[b].y * f;
     }
-    const uint32_t h = self.head_of(c.vh, column);
-    if (d < dim)
-      (static_cast<T*>(p.a.out.p) + int64_t(c.i) * p.a.out.token_stride + int64_t(h) * p.a.out.head_stride)[d] =
-          Mma<T>::from(l == 0.0f ? 0.0f : o / l);
-    if (d == 0 && p.a.lse)
-      p.a.lse[int64_t(c.i) * p.a.n_q_heads + h] = l == 0.0f ? -INFINITY : (ref + log2f(l)) * 0.6931471805599453f;
+    put(column, d, ref, o, l);
   }
   // no block leaves while another may read its shared memory
   asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
@@ -910,7 +961,7 @@ struct Shape {
   int dp, nt, warps;
   uint32_t group, head_tiles, workers;
   uint64_t row_heads;
-  uint32_t cluster;
+  uint32_t cluster, share;
 };
 Shape shape_of(const AttendArgs& a) {
   Shape s;
@@ -931,8 +982,10 @@ Shape shape_of(const AttendArgs& a) {
   // to 4000 26 / 24.
   const uint64_t wide = uint64_t(a.c.max_pages) * a.c.page_size;
   const uint64_t longest = a.window && a.window < wide ? a.window : wide;
-  s.cluster = s.row_heads <= 15 ? 8 : s.row_heads <= 32 ? 4 : s.row_heads <= 74 ? 2 : s.row_heads <= 148 ? 1 : 0;
-  if (longest * s.dp > kTokensOfBlock * 128 * s.cluster) s.cluster = 0;
+  s.cluster = s.row_heads <= 15 ? 8 : s.row_heads <= 32 ? 4 : s.row_heads <= 74 ? 2 : 1;
+  s.share = s.row_heads <= 148 ? 1 : s.row_heads <= 296 ? 2 : s.row_heads <= 592 ? 4 : 8;
+  const uint64_t most = 148 * (s.dp == 256 ? 6 : 8);  // a warp each
+  if (s.row_heads > most || longest * s.dp * s.share > kTokensOfBlock * 128 * s.cluster) s.cluster = 0;
   return s;
 }
 
@@ -963,7 +1016,11 @@ void launch_typed(const AttendParams& p, cudaStream_t st) {
     using C = Attend<T, DP, NT, ring.warps, ring.stages>;
     auto cluster_kernel = attend_cluster_kernel<T, DP, NT, ring.warps, ring.stages>;
     allow_shared(cluster_kernel, C::kRingBytes, cluster_ready, m);
-    launch("attend", cluster_kernel, dim3(p.cluster, uint32_t(row_heads)), C::kThreads, C::kRingBytes, st, p.cluster, p);
+    AttendParams q = p;
+    q.warps_each = p.share > uint32_t(ring.warps) ? 1 : ring.warps / p.share;
+    const uint32_t groups = ring.warps / q.warps_each;
+    launch("attend", cluster_kernel, dim3(p.cluster, uint32_t((row_heads + groups - 1) / groups)), C::kThreads,
+           C::kRingBytes, st, p.cluster, q);
     return;
   }
   allow_shared(kernel, A::shared_bytes(), ready, m);
@@ -1022,6 +1079,8 @@ void launch_attend(const AttendArgs& a, void* scratch, cudaStream_t st) {
     throw std::invalid_argument("rows, heads and tokens are too many for one call");
   p.by_worker = s.row_heads > s.workers;
   p.cluster = s.cluster;
+  p.share = s.share;
+  p.row_heads = s.row_heads;
   p.tiled_pages = a.c.page_size % TK == 0;
   const size_t slots = size_t(2) * s.workers * 8 * s.nt;
   unsigned char* at = static_cast<unsigned char*>(scratch);
