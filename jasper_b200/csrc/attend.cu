@@ -662,6 +662,7 @@ __global__ void __launch_bounds__(WARPS * 32) attend_kernel(const __grid_constan
 // scratch.
 constexpr int kCluster = 8;                // the largest
 constexpr uint64_t kTokensOfBlock = 1500;  // of heads of 128, at most
+constexpr uint64_t kMostShared = 300000;   // rows' heads: a grid has 65,535 blocks in y
 // Fewer warps start, and are joined, sooner: 1000 tokens of 8 heads of 128
 // took 6.4 us with 8 warps a block, 7.2 with 12, 6.7 with 4; 4000 tokens 9.4,
 // 10.0 and 11.9.
@@ -984,8 +985,7 @@ Shape shape_of(const AttendArgs& a) {
   const uint64_t longest = a.window && a.window < wide ? a.window : wide;
   s.cluster = s.row_heads <= 15 ? 8 : s.row_heads <= 32 ? 4 : s.row_heads <= 74 ? 2 : 1;
   s.share = s.row_heads <= 148 ? 1 : s.row_heads <= 296 ? 2 : s.row_heads <= 592 ? 4 : 8;
-  const uint64_t most = 148 * (s.dp == 256 ? 6 : 8);  // a warp each
-  if (s.row_heads > most || longest * s.dp * s.share > kTokensOfBlock * 128 * s.cluster) s.cluster = 0;
+  if (s.row_heads > kMostShared || longest * s.dp * s.share > kTokensOfBlock * 128 * s.cluster) s.cluster = 0;
   return s;
 }
 

@@ -139,10 +139,23 @@ def test_more_rows_and_heads_than_workers(cuda):
 
 @pytest.mark.parametrize("rows", [1, 8, 9, 16, 17, 37, 38, 74, 75])
 def test_few_rows_in_clusters(cuda, rows):
+    """Clusters of 8, 4, 2 and 1 blocks."""
     lengths = [(61 * i) % 180 for i in range(rows)]
     lengths[-1] = 900
     c = make(lengths, kv_heads=2, dim=64, dtype=torch.bfloat16)
     q = queries(rows, 6, 64, torch.bfloat16)
+    out, lse = c.attend(0, q, return_lse=True)
+    check(c, q, out, lse)
+
+
+@pytest.mark.parametrize("rows,longest", [(75, 700), (148, 600), (149, 300), (296, 150), (297, 180), (600, 90)])
+@pytest.mark.parametrize("dim,group", [(64, 3), (128, 16), (256, 2), (96, 9)])
+def test_rows_that_share_blocks(cuda, rows, longest, dim, group):
+    """All, four, two or one of a block's warps to a row's head; some rows are empty."""
+    lengths = [(53 * i) % (longest + 1) for i in range(rows)]
+    lengths[0] = longest
+    c = make(lengths, kv_heads=1, dim=dim, page_size=32, dtype=torch.bfloat16)
+    q = queries(rows, group, dim, torch.bfloat16)
     out, lse = c.attend(0, q, return_lse=True)
     check(c, q, out, lse)
 
