@@ -201,24 +201,33 @@ struct Wants {
   }
 };
 
-// Finds the lowest free pages and calls give(rank, page) for each rank below
-// `total`; `bits0` are the thread's free pages of its first turn, `before` the
-// free pages of the blocks below.  The pages go through a list (kBlockPages
-// entries), so that each is a thread's of its own: a thread that gave its 16
-// away one by one took 4 us.
+// Finds the lowest free pages and calls give(row of the call, rank, page) for
+// each rank below `total`; `bits0` are the thread's free pages of its first
+// turn, `before` the free pages of the blocks below.  The pages go through a
+// list (kBlockPages entries), so that each is a thread's of its own: a thread
+// that gave its 16 away one by one took 4 us.  The row is searched for at
+// kMarks ranks only, and stepped to between.
+constexpr int kMarks = kPlanThreads;
 template <typename F>
 __device__ __forceinline__ void hand_out(const jb_page_cache& c, const PoolPart& part, uint32_t bits0, int before,
-                                         int total, uint16_t* list, F&& give) {
+                                         int total, const Wants& w, uint32_t n_rows, F&& give) {
+  __shared__ int marks[kMarks];
   for (uint32_t turn = 0; turn < part.turns() && before < total; turn++) {
     const uint32_t first = part.first(turn), base = part.begin + turn * kBlockPages;
     uint32_t bits = turn == 0 ? bits0 : free_bits(c, part, first);
     int all;
     const int n = __popc(bits);
     int at = block_scan(n, &all) - n;
-    for (; bits; bits &= bits - 1) list[at++] = uint16_t(first - base + __ffs(bits) - 1);
+    for (; bits; bits &= bits - 1) w.free_list[at++] = uint16_t(first - base + __ffs(bits) - 1);
+    const int count = min(all, total - before);
+    const int shift = max(0, 22 - __clz(count - 1 | 1));  // count <= kMarks << shift
+    if (int(threadIdx.x) << shift < count) marks[threadIdx.x] = w.row_of(before + (int(threadIdx.x) << shift), n_rows);
     __syncthreads();
-    for (int i = threadIdx.x; i < min(all, total - before); i += kPlanThreads)
-      give(before + i, int32_t(base + list[i]));
+    for (int k = threadIdx.x; k < count; k += kPlanThreads) {
+      int i = marks[k >> shift];
+      while (w.upto[i] <= before + k) i++;
+      give(uint32_t(i), before + k, int32_t(base + w.free_list[k]));
+    }
     __syncthreads();
     before += all;
   }
@@ -278,8 +287,7 @@ extend_kernel(const jb_page_cache c, const int32_t* rows, const int32_t* tokens,
   int before;
   cluster_wait<BLOCKS>();
   const int n_free = exchange<BLOCKS>(count_free(c, part, bits), box, &before);  // all lengths are read behind this
-  hand_out(c, part, bits, before, min(total, n_free), w.free_list, [&](int rank, int32_t page) {
-    const uint32_t i = w.row_of(rank, n);
+  hand_out(c, part, bits, before, min(total, n_free), w, n, [&](uint32_t i, int rank, int32_t page) {
     if (w.upto[i] > n_free) return;
     const int into = rank - (i ? w.upto[i - 1] : 0);
     c.table[w.row[i] * c.table_stride + w.have[i] + into] = page;
@@ -350,8 +358,7 @@ fork_kernel(const jb_page_cache c, const int32_t* parents, const int32_t* childr
   int before;
   cluster_wait<BLOCKS>();
   const int n_free = exchange<BLOCKS>(count_free(c, part, bits), box, &before);  // rows are read, and copies set, behind this
-  hand_out(c, part, bits, before, min(total, n_free), w.free_list, [&](int rank, int32_t page) {
-    const uint32_t i = w.row_of(rank, n);
+  hand_out(c, part, bits, before, min(total, n_free), w, n, [&](uint32_t i, int, int32_t page) {
     c.table[w.row[i] * c.table_stride + uint32_t(w.have[i]) / c.page_size] = page;
     c.refs[page] = 1;
     to_of[i] = page;
