@@ -373,7 +373,8 @@ fork_kernel(const jb_page_cache c, const int32_t* parents, const int32_t* childr
   }
 }
 
-__global__ void __launch_bounds__(256)
+constexpr int kFreeThreads = 256;
+__global__ void __launch_bounds__(kFreeThreads)
 free_kernel(const jb_page_cache c, const int32_t* rows) {
   follow();
   const uint32_t i = blockIdx.x;
@@ -383,11 +384,22 @@ free_kernel(const jb_page_cache c, const int32_t* rows) {
     return;
   }
   int32_t* row = c.table + r * c.table_stride;
-  for (uint32_t j = threadIdx.x; j < c.max_pages; j += blockDim.x) {
+  // four entries of a thread at once, for the latency of three dependent steps
+  constexpr int kAtOnce = 4;
+  for (uint64_t j0 = threadIdx.x; j0 < c.max_pages; j0 += kAtOnce * kFreeThreads) {
+    int32_t p[kAtOnce];
+#pragma unroll
+    for (int k = 0; k < kAtOnce; k++) {
+      const uint64_t j = j0 + k * kFreeThreads;
+      p[k] = j < c.max_pages ? row[j] : -1;
+    }
     // exchanged, so that a row named twice gives its pages back once
-    if (row[j] < 0) continue;
-    const int32_t p = atomicExch(row + j, -1);
-    if (page_ok(c, p)) atomicSub(c.refs + p, 1);
+#pragma unroll
+    for (int k = 0; k < kAtOnce; k++)
+      if (p[k] >= 0) p[k] = atomicExch(row + j0 + k * kFreeThreads, -1);
+#pragma unroll
+    for (int k = 0; k < kAtOnce; k++)
+      if (page_ok(c, p[k])) atomicSub(c.refs + p[k], 1);
   }
   if (threadIdx.x == 0) c.lengths[r] = 0;
 }
@@ -657,7 +669,7 @@ void launch_fork(const jb_page_cache& c, const int32_t* parents, const int32_t* 
 
 void launch_free(const jb_page_cache& c, const int32_t* rows, uint32_t n, cudaStream_t st) {
   if (n == 0) return;
-  launch("free", free_kernel, dim3(n), 256, 0, st, 0, c, rows);
+  launch("free", free_kernel, dim3(n), kFreeThreads, 0, st, 0, c, rows);
 }
 
 void launch_adopt(const jb_page_cache& c, const int32_t* rows, const int32_t* pages,
