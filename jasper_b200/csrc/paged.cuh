@@ -96,6 +96,9 @@ struct AppendArgs {
 };
 void launch_append(const AppendArgs& a, cudaStream_t st);
 
+// Throws if the copies of n pages cannot be counted in 32 bits; before a call
+// that copies pages changes anything.
+void check_copies(const jb_page_cache& c, uint64_t n);
 // The page operations' scratch, in int32 words.
 size_t pages_plan_words(const jb_page_cache& c, uint64_t n);
 void launch_extend(const jb_page_cache& c, const int32_t* rows, const int32_t* tokens, uint32_t n,

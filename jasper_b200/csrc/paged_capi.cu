@@ -174,6 +174,7 @@ int jb_pages_fork(const jb_page_cache* cache, const int32_t* parents, const int3
     const jb_page_cache& c = checked(cache);
     if (n == 0) return;
     require(parents && children, "null pointer argument");
+    jb::check_copies(c, n);
     cudaStream_t st = static_cast<cudaStream_t>(stream);
     OnDevice on(c.device);
     Scratch s(jb::pages_plan_words(c, n) * sizeof(int32_t), st);
@@ -213,6 +214,7 @@ int jb_pages_compact(const jb_page_cache* cache, int32_t* remap, void* stream) {
     const jb_page_cache& c = checked(cache);
     if (c.n_pages == 0) return;
     require(remap != nullptr, "null pointer argument");
+    jb::check_copies(c, c.n_pages);
     cudaStream_t st = static_cast<cudaStream_t>(stream);
     OnDevice on(c.device);
     Scratch s(jb::pages_plan_words(c, 0) * sizeof(int32_t), st);
@@ -226,6 +228,7 @@ int jb_pages_copy(const jb_page_cache* cache, const int32_t* src, const int32_t*
     const jb_page_cache& c = checked(cache);
     if (n == 0) return;
     require(src && dst, "null pointer argument");
+    jb::check_copies(c, n);
     OnDevice on(c.device);
     jb::launch_copy_pages(c, src, dst, n, static_cast<cudaStream_t>(stream));
   });

@@ -550,15 +550,14 @@ __global__ void __launch_bounds__(kCopyThreads, 3) copy_pages_kernel(const __gri
       }
       if (lane == 0 && len % int32_t(c.page_size) && a.src[i] < 0) to[whole] = -1;
     }
-  const uint32_t pairs = a.n_device ? uint32_t(max(*a.n_device, 0)) : a.n;
+  const uint32_t pairs = a.n_device ? min(uint32_t(max(*a.n_device, 0)), a.n) : a.n;
   const uint32_t planes = 2 * c.n_layers, row = c.head_dim / 8;  // 16-byte vectors of a head
   const uint32_t full = c.page_size * c.n_kv_heads * row;
   const uint32_t run = a.run * 32 * kCopyDepth, runs = (full + run - 1) / run;
-  const uint64_t units = uint64_t(pairs) * planes * runs;
-  for (uint64_t unit = warp; unit < units; unit += step) {
-    const uint64_t item = unit / runs;
-    const uint32_t i = uint32_t(item / planes), plane = uint32_t(item - uint64_t(i) * planes);
-    const uint32_t begin = uint32_t(unit - item * runs) * run;
+  const uint32_t units = pairs * planes * runs;  // below 2^31: check_copies()
+  for (uint32_t unit = uint32_t(warp); unit < units; unit += uint32_t(step)) {
+    const uint32_t item = unit / runs, i = item / planes, plane = item - i * planes;
+    const uint32_t begin = (unit - item * runs) * run;
     const int32_t from = a.src[i], to = a.dst[i];
     const uint32_t nt = a.tokens ? uint32_t(a.tokens[i]) : c.page_size;
     if (!page_ok(c, from) || !page_ok(c, to)) {
@@ -600,7 +599,6 @@ void launch_copies(CopyArgs a, cudaStream_t st) {
   a.by_head = c.token_stride == dim;
   a.flat = token_rows || (a.by_head && a.tokens == nullptr && c.head_stride == ps * dim);
   const uint64_t full = uint64_t(c.page_size) * c.n_kv_heads * (c.head_dim / 8);
-  if (full > 0x7FFFFFFFull) throw std::invalid_argument("a page is too large");
   constexpr uint64_t kMost = 148 * 8;
   const uint64_t pieces = (full + 32 * kCopyDepth - 1) / (32 * kCopyDepth);
   uint64_t units = uint64_t(a.n) * 2 * c.n_layers * pieces;
@@ -639,6 +637,13 @@ void launch_plan_of(const char* what, cudaStream_t st, A... args) {
   } while (0)
 
 }  // namespace
+
+// What the copies count in 32 bits.
+void check_copies(const jb_page_cache& c, uint64_t n) {
+  if (uint64_t(c.page_size) * c.n_kv_heads * (c.head_dim / 8) > 0x7FFFFFFFull)
+    throw std::invalid_argument("a page is too large");
+  if (n * 2 * c.n_layers > (uint64_t(1) << 30)) throw std::invalid_argument("too many pages for one call");
+}
 
 size_t pages_plan_words(const jb_page_cache& c, uint64_t n) {
   const size_t lists = c.n_rows > kOwnersInBlock || n > kRowsInBlock ? kPlanBlocks * (size_t(c.n_rows) + 4 * size_t(n)) : 0;

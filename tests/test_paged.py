@@ -92,6 +92,11 @@ def test_refused_arguments():
                         ({"dim": 0}, "head_dim"), ({"freq": None}, "null"), ({"pos": None}, "null")):
         with pytest.raises(ValueError, match=message):
             _lib.call("jb_rotary", *{**ro, **kw}.values())
+    for name in ("jb_pages_fork", "jb_pages_copy"):
+        with pytest.raises(ValueError, match="too many pages"):
+            _lib.call(name, cache(n_layers=2 ** 20), 4096, 4096, 1025, None)
+        with pytest.raises(ValueError, match="too large"):
+            _lib.call(name, cache(page_size=2 ** 20, n_kv_heads=65536), 4096, 4096, 1, None)
     with pytest.raises(ValueError, match="more pages"):
         _lib.call("jb_pages_adopt", cache(), 4096, 4096, 5, 5, None, 1, None)
 
