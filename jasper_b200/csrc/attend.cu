@@ -22,12 +22,18 @@
 //  * Products run on mma.sync m16n8k16 with tokens (then head elements) as the
 //    16 rows and query heads as the 8 columns, S^T = K Q^T and O^T = V^T P^T,
 //    so a group of 8 heads wastes nothing; movmatrix turns the weights from
-//    accumulator to operand.  tcgen05 has nothing to give here: its smallest
-//    tile is 64 rows or columns of queries wide, and the tensor pipe is far
-//    from busy.
+//    accumulator to operand.  tcgen05 would take tiles of 64 or 128 tokens,
+//    shared by warps, and the weights through tensor memory and back; the
+//    tensor pipe is 15 % busy here, so it has nothing to give.
 //  * A weight enters the second product as the sum of two 16-bit values (its
 //    rounding, and the rounding of what that left), so nothing is lost
 //    against float32 weights; l sums the float32 weights.
+//  * Short rows take no part in this: warps, blocks or clusters of blocks have
+//    a row's head each, and join in (distributed) shared memory.
+//
+// Measured: 64 rows of 1 to 8191 tokens, 8 heads of 128, bfloat16, 167 us, 6.4
+// TB/s (0.99 of the measured copy rate); 400 k + 333 k tokens, float16, 442 us,
+// 6.8 TB/s; one row of 1000 tokens 5.9 us.
 #include <cmath>
 #include <mutex>
 #include <stdexcept>
