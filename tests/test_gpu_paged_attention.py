@@ -160,6 +160,18 @@ def test_rows_that_share_blocks(cuda, rows, longest, dim, group):
     check(c, q, out, lse)
 
 
+@pytest.mark.parametrize("kv_heads", [1, 2])
+def test_more_queries_than_a_block_lists(cuda, kv_heads):
+    """Over 1024 rows of very different lengths, named in another order."""
+    lengths = [(7 * i) % 50 for i in range(1100)]
+    lengths[700], lengths[3], lengths[1099] = 3000, 700, 260
+    c = make(lengths, kv_heads=kv_heads, dim=64, page_size=16)
+    rows = torch.randperm(1100, generator=torch.Generator().manual_seed(11)).tolist() + [700, -5, 3]
+    q = queries(len(rows), 2 * kv_heads, 64, torch.float16)
+    out, lse = c.attend(0, q, torch.tensor(rows, dtype=torch.int32, device="cuda"), return_lse=True)
+    check(c, q, out, lse, rows=rows)
+
+
 def test_many_short_rows(cuda):
     lengths = [(7 * i) % 50 for i in range(1100)]
     c = make(lengths, kv_heads=1, dim=8, page_size=8)

@@ -26,7 +26,7 @@ def make(n_pages=40, page_size=4, rows=12, width=8, layers=2, kv_heads=2, dim=16
 
 
 def both(c, m, name, *args):
-    r = getattr(c, name)(*(torch.as_tensor(np.asarray(a, np.int32)).cuda() for a in args))
+    r = getattr(c, name)(*(torch.as_tensor(np.ascontiguousarray(a, np.int32)).cuda() for a in args))
     want = getattr(m, name)(*(np.asarray(a, np.int32) for a in args))
     m.check_against(c)
     return r, want
@@ -126,6 +126,25 @@ def test_pools_of_any_size(cuda, n_pages):
     assert torch.equal(remap[moved], holes.int())
     assert torch.equal(c.refs.cpu()[holes], want[moved])
     assert torch.equal(c.table.cpu()[table >= 0], remap[table[table >= 0].long()])
+
+
+@pytest.mark.parametrize("rows,named,n_pages", [(9000, 1500, 9000), (3000, 2900, 5000), (12_000, 5000, 40_000)])
+def test_many_rows(cuda, rows, named, n_pages):
+    """More rows, in the table and in a call, than a block's shared memory keeps."""
+    rng = np.random.default_rng(rows)
+    c, m = make(n_pages, 2, rows, 9, layers=1, kv_heads=1, dim=8)
+    order = rng.permutation(rows)[:named].astype(np.int32)
+    order[5] = order[900]                                   # named twice: the first time counts
+    both(c, m, "extend", order, rng.integers(0, 9, named))
+    both(c, m, "extend", order[::-1], rng.integers(0, 3, named))
+    children = np.setdiff1d(np.arange(rows), order)
+    children = rng.permutation(children)[:min(named // 2, len(children))]
+    parents = rng.choice(order, len(children))
+    both(c, m, "fork", parents, children)
+    both(c, m, "free", order[:named // 3])
+    r, want = both(c, m, "compact")
+    np.testing.assert_array_equal(r.cpu().numpy(), want)
+    both(c, m, "adopt", order[:named // 3], rng.integers(-1, n_pages, (named // 3, 4)))
 
 
 @pytest.mark.parametrize("layout", ["token", "head"])
