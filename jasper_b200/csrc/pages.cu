@@ -617,6 +617,7 @@ void launch_plan_of(const char* what, cudaStream_t st, A... args) {
   static uint64_t ready = 0;
   int dev = 0;
   cudaError_t e = cudaGetDevice(&dev);
+  if (dev >= 64) throw std::runtime_error("device index out of range");
   {
     std::lock_guard<std::mutex> lock(m);
     if (e == cudaSuccess && !(ready >> dev & 1)) {
