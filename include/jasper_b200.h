@@ -367,7 +367,9 @@ int jb_merge_topk_strided(const int32_t* shard_idx, const float* shard_dist, uin
  * conversation) holds lengths[row] tokens in the pages table[row][0 ..
  * ceil(length / page_size)); an entry of -1 is a page that is not there: its
  * tokens are never attended to.  refs[page] counts the rows that hold a page;
- * 0 is free. */
+ * 0 is free.  marks[row] is negative while the row's last jb_pages_extend was
+ * refused: its last token is then an old one, and jb_kv_append without index
+ * leaves it alone.  Set it to 0 for a row whose length you set yourself. */
 typedef struct jb_page_cache {
   void* k;
   void* v;
@@ -375,6 +377,7 @@ typedef struct jb_page_cache {
   int32_t* lengths; /* [n_rows] */
   int32_t* refs;    /* [n_pages] */
   int32_t* status;  /* one word of JB_PAGES_* bits */
+  int32_t* marks;   /* [n_rows], zeros at first: what the calls note of a row; or NULL */
   int64_t layer_stride, page_stride, token_stride, head_stride;
   int64_t table_stride;
   uint32_t n_layers, n_pages, page_size, n_kv_heads, head_dim;
@@ -403,7 +406,8 @@ int jb_rotary(const void* x, int64_t x_token_stride, int64_t x_head_stride, void
 /* Writes n_tokens new keys and values ([n_tokens][n_kv_heads][head_dim] of the
  * cache's type, any token and head stride) into one layer: token t becomes
  * token index[t] of row rows[t] (index NULL: the row's last, lengths[row] -
- * 1).  With freq, keys are rotated on the way as by jb_rotary (positions NULL:
+ * 1, which needs the cache's marks: a row that jb_pages_extend refused room has
+ * no place for a new token).  With freq, keys are rotated on the way as by jb_rotary (positions NULL:
  * the token's index), and with q so are n_q_heads query heads, into q_out
  * (which may be q).  The page must not be shared with a row that still needs
  * its old tokens there (jb_pages_fork sees to that).  A token whose place
@@ -422,7 +426,8 @@ int jb_kv_append(const jb_page_cache* cache, uint32_t layer, uint64_t n_tokens, 
  * one is full (the free pages with the lowest numbers, in the order of the
  * rows), and a length that counts them.  Rows are served in order until the
  * free pages run out; from the first that finds too few on, rows that need
- * pages are left as they were (JB_PAGES_EXHAUSTED). */
+ * pages are left as they were (JB_PAGES_EXHAUSTED).  Rows that are left as they
+ * were, for that or another reason, are marked. */
 int jb_pages_extend(const jb_page_cache* cache, const int32_t* rows, const int32_t* tokens,
                     uint32_t n, void* stream);
 

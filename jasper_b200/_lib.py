@@ -39,7 +39,7 @@ class PageCache(C.Structure):
     """jb_page_cache."""
     _fields_ = [
         ("k", C.c_void_p), ("v", C.c_void_p), ("table", C.c_void_p), ("lengths", C.c_void_p),
-        ("refs", C.c_void_p), ("status", C.c_void_p),
+        ("refs", C.c_void_p), ("status", C.c_void_p), ("marks", C.c_void_p),
         ("layer_stride", C.c_int64), ("page_stride", C.c_int64), ("token_stride", C.c_int64),
         ("head_stride", C.c_int64), ("table_stride", C.c_int64),
         ("n_layers", C.c_uint32), ("n_pages", C.c_uint32), ("page_size", C.c_uint32),

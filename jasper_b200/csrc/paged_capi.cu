@@ -137,6 +137,7 @@ int jb_kv_append(const jb_page_cache* cache, uint32_t layer, uint64_t n_tokens, 
     if (n_tokens == 0) return;
     require(k && v && rows, "null pointer argument");
     require(!q || (q_out && freq), "q needs q_out and freq");
+    require(index || a.c.marks, "without index the cache's marks are needed");
     a.layer = layer;
     a.n_tokens = n_tokens;
     if (q) {

@@ -294,11 +294,17 @@ extend_kernel(const jb_page_cache c, const int32_t* rows, const int32_t* tokens,
     c.refs[page] = 1;
   });
   if (!speaks) return;
+  // A row that stays as it was is marked, so that an append to its last token
+  // does not take the place of an old one.
   for (uint32_t i = threadIdx.x; i < n; i += blockDim.x) {
-    if (w.have[i] < 0) continue;
-    const bool none = pages_for(uint32_t(w.extra[i]), c.page_size) <= uint32_t(w.have[i]);
-    if (none || w.upto[i] <= n_free) c.lengths[w.row[i]] = w.extra[i];
-    else atomicOr(c.status, kPagesExhausted);
+    const int32_t r = w.row[i];
+    if (!row_ok(c, r) || w.owner[r] != int32_t(i)) continue;
+    const bool ok = w.have[i] >= 0;
+    const bool none = ok && pages_for(uint32_t(w.extra[i]), c.page_size) <= uint32_t(w.have[i]);
+    const bool given = none || (ok && w.upto[i] <= n_free);
+    if (given) c.lengths[r] = w.extra[i];
+    else if (ok) atomicOr(c.status, kPagesExhausted);
+    if (c.marks) c.marks[r] = given ? 0 : kMarkRefused;
   }
 }
 
@@ -316,7 +322,7 @@ fork_kernel(const jb_page_cache c, const int32_t* parents, const int32_t* childr
   const uint32_t bits = free_bits(c, part, part.first(0));
   Wants w(c, n, shared, scratch);
   struct Turn {
-    int32_t child = -1, len = -1, from = -1;  // len -1: no pair to fork
+    int32_t child = -1, len = -1, from = -1, mark = 0;  // len -1: no pair to fork
     __device__ Turn(const jb_page_cache& c, const int32_t* parents, const int32_t* children, uint32_t i, uint32_t n) {
       if (i >= n) return;
       const int32_t p = parents[i];
@@ -325,6 +331,7 @@ fork_kernel(const jb_page_cache c, const int32_t* parents, const int32_t* childr
       const int32_t held = row_ok(c, p) ? max(c.lengths[p], 0) : -1;
       if (there != 0 || held < 0 || pages_for(uint32_t(held), c.page_size) > c.max_pages) return;
       len = held;
+      if (c.marks) mark = c.marks[p];
       const uint32_t whole = uint32_t(len) / c.page_size;
       if (whole * c.page_size == uint32_t(len)) return;
       from = c.table[p * c.table_stride + whole];
@@ -368,8 +375,14 @@ fork_kernel(const jb_page_cache c, const int32_t* parents, const int32_t* childr
     const int32_t len = w.have[i];
     const bool given = len >= 0 && (w.extra[i] < 0 || w.upto[i] <= n_free);
     length_of[i] = given ? len : -1;
-    if (given) c.lengths[w.row[i]] = len;
-    else if (len >= 0) atomicOr(c.status, kPagesExhausted);
+    if (given) {
+      c.lengths[w.row[i]] = len;
+      // a refused parent's last token is an old one in its child too; a parent
+      // that is another pair's child is empty, and its mark does not matter
+      if (c.marks) c.marks[w.row[i]] = (i == threadIdx.x ? first.mark : c.marks[parents[i]]) & kMarkRefused;
+    } else if (len >= 0) {
+      atomicOr(c.status, kPagesExhausted);
+    }
   }
 }
 
@@ -401,7 +414,10 @@ free_kernel(const jb_page_cache c, const int32_t* rows) {
     for (int k = 0; k < kAtOnce; k++)
       if (page_ok(c, p[k])) atomicSub(c.refs + p[k], 1);
   }
-  if (threadIdx.x == 0) c.lengths[r] = 0;
+  if (threadIdx.x == 0) {
+    c.lengths[r] = 0;
+    if (c.marks) c.marks[r] = 0;
+  }
 }
 
 // owner[row] = the first i that names the row
@@ -438,7 +454,10 @@ adopt_kernel(const jb_page_cache c, const int32_t* rows, const int32_t* pages, i
     if (is) atomicAdd(c.refs + p, 1);
     else if (p != -1) atomicOr(c.status, kPagesBadToken);
   }
-  if (threadIdx.x == 0) c.lengths[r] = int32_t(len);
+  if (threadIdx.x == 0) {
+    c.lengths[r] = int32_t(len);
+    if (c.marks) c.marks[r] = 0;
+  }
 }
 
 // moves[0]: how many; then the pages that move and, n_pages on, where to.

@@ -135,7 +135,10 @@ __global__ void __launch_bounds__(kMaxThreads, kBlocks) rotary_kernel(const __gr
     const int32_t row = a.rows[t];
     int64_t to = -1;
     if (row >= 0 && uint32_t(row) < a.c.n_rows) {
-      const int64_t i = a.index ? int64_t(a.index[t]) : int64_t(a.c.lengths[row]) - 1;
+      // a row that was refused room has no new last token
+      const int64_t i = a.index                          ? int64_t(a.index[t])
+                        : a.c.marks[row] & kMarkRefused ? int64_t(-1)
+                                                         : int64_t(a.c.lengths[row]) - 1;
       if (i >= 0 && uint32_t(i) / a.c.page_size < a.c.max_pages) {
         const uint32_t pg = uint32_t(i) / a.c.page_size, slot = uint32_t(i) % a.c.page_size;
         const int32_t page = a.c.table[row * a.c.table_stride + pg];

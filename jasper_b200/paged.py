@@ -140,11 +140,14 @@ class PagedCache:
     them).  ``table`` int32 [rows, max_pages]: a row's pages, -1 for none;
     ``lengths`` int32 [rows]; ``refs`` int32 [pages]: how many rows hold a
     page (0: free).  The tensors stay the caller's: the cache changes them in
-    place, and a program may read or write them between calls.
+    place, and a program may read or write them between calls.  ``marks`` int32
+    [rows] (made here if not given) is what the calls note of a row: negative
+    while its last extend() was refused, so that append() does not write over
+    its last token; 0 for a row whose length the program sets itself.
     """
 
     def __init__(self, k: torch.Tensor, v: torch.Tensor, table: torch.Tensor, lengths: torch.Tensor,
-                 refs: torch.Tensor, status: torch.Tensor | None = None):
+                 refs: torch.Tensor, status: torch.Tensor | None = None, marks: torch.Tensor | None = None):
         if not k.is_cuda:
             raise ValueError("k must be a CUDA tensor")
         device = k.device
@@ -166,20 +169,26 @@ class PagedCache:
             status = torch.zeros(1, dtype=torch.int32, device=device)
         elif status.numel() != 1:
             raise ValueError(f"status must have one element, got {status.numel()}")
-        for t, name in ((table, "table"), (lengths, "lengths"), (refs, "refs"), (status, "status")):
+        if marks is None:
+            marks = torch.zeros(table.size(0), dtype=torch.int32, device=device)
+        elif marks.shape != (table.size(0),) or not marks.is_contiguous():
+            raise ValueError(f"marks must be a contiguous [{table.size(0)}]")
+        for t, name in ((table, "table"), (lengths, "lengths"), (refs, "refs"), (status, "status"),
+                        (marks, "marks")):
             if t.dtype != torch.int32:
                 raise ValueError(f"{name} must be int32, got {t.dtype}")
         for t, name in ((v, "v"), (table, "table"), (lengths, "lengths"), (refs, "refs"),
-                        (status, "status")):
+                        (status, "status"), (marks, "marks")):
             if t.device != device:
                 raise ValueError(f"{name} must be on {device}, got {t.device}")
         self.k, self.v, self.table, self.lengths, self.refs, self.status = k, v, table, lengths, refs, status
+        self.marks = marks
         self.device, self.dtype = device, k.dtype
         self.n_layers, self.n_pages, self.page_size, self.n_kv_heads, self.head_dim = k.shape
         self.n_rows, self.max_pages = table.shape
         self._c = _lib.PageCache(
             k.data_ptr(), v.data_ptr(), table.data_ptr(), lengths.data_ptr(), refs.data_ptr(),
-            status.data_ptr(), *k.stride()[:4], table.stride(0), *k.shape, *table.shape,
+            status.data_ptr(), marks.data_ptr(), *k.stride()[:4], table.stride(0), *k.shape, *table.shape,
             _DTYPES[k.dtype], device.index)
         self._ref = C.addressof(self._c)
         self._native = _lib.paged_module()
@@ -209,7 +218,8 @@ class PagedCache:
         """Room for ``tokens[i]`` more tokens in row ``rows[i]``: pages where
         its last one is full (the lowest free ones), and a length that counts
         them.  Rows are served in order; from the first that finds too few
-        free pages on, rows that need pages stay as they were."""
+        free pages on, rows that need pages stay as they were, and append()
+        leaves their last token alone until they are extended."""
         self._native.extend(self._ref, rows, tokens)
 
     def fork(self, parents: torch.Tensor, children: torch.Tensor) -> None:
@@ -244,7 +254,7 @@ class PagedCache:
                q_out: torch.Tensor | None = None) -> torch.Tensor | None:
         """Writes keys and values [tokens, kv_heads, head_dim] as tokens
         ``index`` (default: each row's last) of rows ``rows`` (extend() made
-        the room).  With ``rotary``, keys are turned by ``positions`` (default:
+        the room; a token of a row that it refused is not written).  With ``rotary``, keys are turned by ``positions`` (default:
         the index) on the way, and so is ``q`` [tokens, heads, head_dim], which
         is returned (in ``q_out`` if given, which may be ``q``)."""
         r = (None, 0, 0, 1.0, False) if rotary is None else rotary._args
