@@ -367,9 +367,12 @@ int jb_merge_topk_strided(const int32_t* shard_idx, const float* shard_dist, uin
  * conversation) holds lengths[row] tokens in the pages table[row][0 ..
  * ceil(length / page_size)); an entry of -1 is a page that is not there: its
  * tokens are never attended to.  refs[page] counts the rows that hold a page;
- * 0 is free.  marks[row] is negative while the row's last jb_pages_extend was
- * refused: its last token is then an old one, and jb_kv_append without index
- * leaves it alone.  Set it to 0 for a row whose length you set yourself. */
+ * 0 is free.  marks[row] has its sign set while the row's last jb_pages_extend
+ * was refused: its last token is then an old one, and jb_kv_append without index
+ * leaves it alone.  Its other bits are the length that jb_pages_adopt gave the
+ * row, if that ends inside a page: the rest of that page belongs to others, so
+ * the row's tokens there are neither written nor attended to.  Set a mark to 0
+ * for a row whose length and pages you set yourself. */
 typedef struct jb_page_cache {
   void* k;
   void* v;
@@ -445,7 +448,10 @@ int jb_pages_free(const jb_page_cache* cache, const int32_t* rows, uint32_t n, v
 /* Gives the empty row rows[i] the first ceil(lengths[i] / page_size) of the m
  * pages at pages + i * pages_stride as further holder (a search's ids, or
  * another row's pages; -1 and, with JB_PAGES_BAD_TOKEN, numbers out of range
- * stand for pages that are not there).  lengths NULL: m whole pages each. */
+ * stand for pages that are not there).  lengths NULL: m whole pages each;
+ * lengths need the cache's marks.  A row that ends inside a page shares it with
+ * its other holders, who may still fill it: to go on behind such a row, fork it,
+ * which copies the tokens that it has there. */
 int jb_pages_adopt(const jb_page_cache* cache, const int32_t* rows, const int32_t* pages,
                    int64_t pages_stride, uint32_t m, const int32_t* lengths, uint32_t n,
                    void* stream);
@@ -469,8 +475,9 @@ int jb_pages_copy(const jb_page_cache* cache, const int32_t* src, const int32_t*
  * has no tokens).  Tokens that are not attended to: those of pages that are
  * not there, those t < mask_width with mask[i * mask_stride + t] = 0 (bytes;
  * NULL: none), and with window > 0 all but the row's last `window`.  What
- * their keys and values hold does not matter.  q and out: [n][n_q_heads][head_dim] of the
- * cache's type at any stride that is a multiple of 16 bytes.  lse (float32
+ * their keys and values hold does not matter.  Nor are those attended to that
+ * lie in the rest of a page in which jb_pages_adopt ended.  q and out:
+ * [n][n_q_heads][head_dim] of the cache's type at any stride that is a multiple of 16 bytes.  lse (float32
  * [n][n_q_heads], or NULL): log sum exp of the scaled scores, with which parts
  * of one attention can be joined.  A query with nothing to attend to gives
  * zeros, and lse -inf. */

@@ -153,7 +153,15 @@ struct AttendParams {
 // The tiles of TK tokens that query i reads.
 struct Tiles {
   int32_t row, len, first, begin, end;
+  uint32_t gap, gap_len;  // tokens that lie in the rest of a page in which the row was adopted: not its own
+  __device__ __forceinline__ void set_gap(const jb_page_cache& c, int32_t adopted) {
+    gap = uint32_t(adopted);
+    gap_len = adopted ? (c.page_size - gap % c.page_size) % c.page_size : 0;
+  }
 };
+__device__ __forceinline__ int32_t adopted_length(const jb_page_cache& c, int32_t row) {
+  return c.marks && row >= 0 && uint32_t(row) < c.n_rows ? c.marks[row] & kMarkAdopted : 0;
+}
 __device__ __forceinline__ Tiles tiles_of(const AttendArgs& a, uint32_t i) {
   Tiles t;
   t.row = a.rows ? a.rows[i] : int32_t(i);
@@ -164,6 +172,7 @@ __device__ __forceinline__ Tiles tiles_of(const AttendArgs& a, uint32_t i) {
   t.first = a.window && len > int64_t(a.window) ? int32_t(len - a.window) : 0;
   t.begin = t.first / TK;
   t.end = int32_t((len + TK - 1) / TK);
+  t.set_gap(a.c, adopted_length(a.c, t.row));
   return t;
 }
 
@@ -258,14 +267,14 @@ struct Attend {
   static constexpr int kStageBytes = 2 * kTileBytes;
   static constexpr int kRingBytes = WARPS * STAGES * kStageBytes;
   static constexpr int shared_bytes() {
-    return kRingBytes + WARPS * STAGES * 4 + kMaxListed * 8 + (kMaxListed + 1) * 8 + 8;
+    return kRingBytes + WARPS * STAGES * 4 + kMaxListed * 12 + (kMaxListed + 1) * 8 + 8;
   }
   static constexpr int KS = DP / 16;                     // k steps of Q K, head tiles of 16 of P V
   static constexpr int kChunkLanes = DP <= 64 ? 8 : DP <= 128 ? 16 : 32;  // lanes a row of 16-byte chunks takes
   static constexpr int kRowsPerCopy = 32 / kChunkLanes;
 
   struct Lists {
-    int32_t *row, *len;
+    int32_t *row, *len, *adopted;
     int64_t* prefix;
   };
 
@@ -281,6 +290,7 @@ struct Attend {
     t.first = p.a.window && t.len > int64_t(p.a.window) ? int32_t(t.len - p.a.window) : 0;
     t.begin = t.first / TK;
     t.end = int32_t((int64_t(t.len) + TK - 1) / TK);
+    t.set_gap(p.a.c, lists.adopted[i]);
     return t;
   }
   __device__ __forceinline__ uint32_t head_rows() const { return p.a.c.n_kv_heads * p.head_tiles; }
@@ -307,7 +317,7 @@ struct Attend {
   __device__ __forceinline__ Place place_of(const Cursor& c) const {
     Place x;
     const uint32_t t = uint32_t(c.tile) * TK + (lane & 15);
-    x.seen = int32_t(t) >= c.t.first && int32_t(t) < c.t.len;
+    x.seen = int32_t(t) >= c.t.first && int32_t(t) < c.t.len && t - c.t.gap >= c.t.gap_len;
     if (x.seen && p.a.mask && t < p.a.mask_width) x.seen = p.a.mask[int64_t(c.i) * p.a.mask_stride + t];
     const uint32_t at = p.tiled_pages ? uint32_t(c.tile) * TK : min(t, uint32_t(c.t.len) - 1);
     const uint32_t pg = at / p.a.c.page_size;
@@ -612,8 +622,8 @@ __global__ void __launch_bounds__(WARPS * 32) attend_kernel(const __grid_constan
   uint32_t* valid = reinterpret_cast<uint32_t*>(smem + A::kRingBytes);
   int64_t* prefix = reinterpret_cast<int64_t*>(smem + ((A::kRingBytes + WARPS * STAGES * 4 + 7) & ~7));
   int32_t* row = reinterpret_cast<int32_t*>(prefix + kMaxListed + 1);
-  int32_t* len = row + kMaxListed;
-  typename A::Lists lists{row, len, prefix};
+  int32_t *len = row + kMaxListed, *adopted = len + kMaxListed;
+  typename A::Lists lists{row, len, adopted, prefix};
   const int wid = threadIdx.x >> 5;
   A self{p, lists, int(threadIdx.x & 31)};
   follow();
@@ -631,6 +641,7 @@ __global__ void __launch_bounds__(WARPS * 32) attend_kernel(const __grid_constan
         const Tiles t = tiles_of(p.a, i);
         row[i] = t.row;
         len[i] = t.len;
+        adopted[i] = adopted_length(p.a.c, t.row);
         v = max(t.end - t.begin, 0);
       }
       int64_t sum;
@@ -687,7 +698,7 @@ __global__ void __launch_bounds__(WARPS * 32) attend_cluster_kernel(const __grid
   __shared__ __align__(16) float block_o[C][DP];
   follow();
   const int wid = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const typename A::Lists none{nullptr, nullptr, nullptr};
+  const typename A::Lists none{};
   const A self{p, none, lane};
   // the warps of a row's head: `each` of a block's, in `blocks` blocks
   const int each = int(p.warps_each), group = wid / each, blocks = int(gridDim.x);

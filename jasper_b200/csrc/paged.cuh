@@ -55,8 +55,10 @@ constexpr int kPagesExhausted = JB_PAGES_EXHAUSTED;
 constexpr int kPagesBadRow = JB_PAGES_BAD_ROW;
 constexpr int kPagesBadToken = JB_PAGES_BAD_TOKEN;
 
-// Bits of a row's mark (jb_page_cache::marks).
-constexpr int32_t kMarkRefused = INT32_MIN;  // its last extend was refused
+// Bits of a row's mark (jb_page_cache::marks): its last extend was refused; and
+// the length at which it was adopted, if that is inside a page.  What follows in
+// that page is not the row's.
+constexpr int32_t kMarkRefused = INT32_MIN, kMarkAdopted = INT32_MAX;
 
 // Rotary positions as the kernels take them: freq[i] is pair i's turn for one
 // position in units of 2^-64 of a turn, so position * freq wraps at whole

@@ -203,6 +203,7 @@ int jb_pages_adopt(const jb_page_cache* cache, const int32_t* rows, const int32_
     require(rows && (pages || m == 0), "null pointer argument");
     require(n < (1u << 30), "too many rows");
     require(m <= c.max_pages, "more pages than a row of the table holds");
+    require(!lengths || c.marks, "with lengths the cache's marks are needed");
     cudaStream_t st = static_cast<cudaStream_t>(stream);
     OnDevice on(c.device);
     Scratch s(size_t(c.n_rows) * sizeof(int32_t), st);

@@ -304,7 +304,9 @@ extend_kernel(const jb_page_cache c, const int32_t* rows, const int32_t* tokens,
     const bool given = none || (ok && w.upto[i] <= n_free);
     if (given) c.lengths[r] = w.extra[i];
     else if (ok) atomicOr(c.status, kPagesExhausted);
-    if (c.marks) c.marks[r] = given ? 0 : kMarkRefused;
+    if (!c.marks) continue;
+    if (!given) atomicOr(c.marks + r, kMarkRefused);
+    else atomicAnd(c.marks + r, w.have[i] == 0 ? 0 : kMarkAdopted);  // an empty row begins anew
   }
 }
 
@@ -377,9 +379,13 @@ fork_kernel(const jb_page_cache c, const int32_t* parents, const int32_t* childr
     length_of[i] = given ? len : -1;
     if (given) {
       c.lengths[w.row[i]] = len;
-      // a refused parent's last token is an old one in its child too; a parent
-      // that is another pair's child is empty, and its mark does not matter
-      if (c.marks) c.marks[w.row[i]] = (i == threadIdx.x ? first.mark : c.marks[parents[i]]) & kMarkRefused;
+      // A refused parent's last token is an old one in its child too.  Where
+      // the parent ends as it was adopted, the child's last page is its own.
+      // A parent that is another pair's child is empty, whatever its mark.
+      if (c.marks) {
+        const int32_t mark = i == threadIdx.x ? first.mark : c.marks[parents[i]], adopted = mark & kMarkAdopted;
+        c.marks[w.row[i]] = (mark & kMarkRefused) | (len > adopted ? adopted : 0);
+      }
     } else if (len >= 0) {
       atomicOr(c.status, kPagesExhausted);
     }
@@ -456,7 +462,7 @@ adopt_kernel(const jb_page_cache c, const int32_t* rows, const int32_t* pages, i
   }
   if (threadIdx.x == 0) {
     c.lengths[r] = int32_t(len);
-    if (c.marks) c.marks[r] = 0;
+    if (c.marks) c.marks[r] = len % ps ? int32_t(len) : 0;
   }
 }
 

@@ -136,10 +136,13 @@ __global__ void __launch_bounds__(kMaxThreads, kBlocks) rotary_kernel(const __gr
     int64_t to = -1;
     if (row >= 0 && uint32_t(row) < a.c.n_rows) {
       // a row that was refused room has no new last token
-      const int64_t i = a.index                          ? int64_t(a.index[t])
-                        : a.c.marks[row] & kMarkRefused ? int64_t(-1)
-                                                         : int64_t(a.c.lengths[row]) - 1;
-      if (i >= 0 && uint32_t(i) / a.c.page_size < a.c.max_pages) {
+      const int32_t mark = a.c.marks ? a.c.marks[row] : 0;
+      const int64_t i = a.index ? int64_t(a.index[t]) : mark < 0 ? int64_t(-1) : int64_t(a.c.lengths[row]) - 1;
+      const uint32_t adopted = uint32_t(mark & kMarkAdopted);
+      // the rest of the page in which it was adopted is not the row's
+      const bool others = adopted % a.c.page_size && i >= int64_t(adopted) &&
+                          uint32_t(i) / a.c.page_size == adopted / a.c.page_size;
+      if (i >= 0 && !others && uint32_t(i) / a.c.page_size < a.c.max_pages) {
         const uint32_t pg = uint32_t(i) / a.c.page_size, slot = uint32_t(i) % a.c.page_size;
         const int32_t page = a.c.table[row * a.c.table_stride + pg];
         if (page >= 0 && uint32_t(page) < a.c.n_pages)

@@ -143,7 +143,8 @@ class PagedCache:
     place, and a program may read or write them between calls.  ``marks`` int32
     [rows] (made here if not given) is what the calls note of a row: negative
     while its last extend() was refused, so that append() does not write over
-    its last token; 0 for a row whose length the program sets itself.
+    its last token; the other bits where adopt() ended inside a page; 0 for a
+    row whose length and pages the program sets itself.
     """
 
     def __init__(self, k: torch.Tensor, v: torch.Tensor, table: torch.Tensor, lengths: torch.Tensor,
@@ -234,7 +235,11 @@ class PagedCache:
     def adopt(self, rows: torch.Tensor, pages: torch.Tensor, lengths: torch.Tensor | None = None) -> None:
         """Makes the empty rows ``rows`` further holders of ``pages`` (int32
         [len(rows), m]; -1: not there), whole or, with ``lengths``, the first
-        lengths[i] tokens of them: a search's ids become rows to attend to."""
+        lengths[i] tokens of them: a search's ids become rows to attend to.  A
+        row that ends so inside a page shares it with holders who may still
+        fill it: what follows in that page is not the row's, append() does not
+        write it and attend() does not read it.  To go on behind such a row
+        fork() it, which copies the tokens that it has there."""
         self._native.adopt(self._ref, rows, pages, lengths)
 
     def compact(self) -> torch.Tensor:
@@ -254,7 +259,8 @@ class PagedCache:
                q_out: torch.Tensor | None = None) -> torch.Tensor | None:
         """Writes keys and values [tokens, kv_heads, head_dim] as tokens
         ``index`` (default: each row's last) of rows ``rows`` (extend() made
-        the room; a token of a row that it refused is not written).  With ``rotary``, keys are turned by ``positions`` (default:
+        the room; a token of a row that it refused, or in the rest of a page
+        that the row was adopted into, is not written).  With ``rotary``, keys are turned by ``positions`` (default:
         the index) on the way, and so is ``q`` [tokens, heads, head_dim], which
         is returned (in ``q_out`` if given, which may be ``q``)."""
         r = (None, 0, 0, 1.0, False) if rotary is None else rotary._args

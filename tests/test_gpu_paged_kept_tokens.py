@@ -132,3 +132,121 @@ def test_marks_of_the_callers_own(cuda):
     for bad in (marks[:1], marks.long(), marks.cpu(), ints(0, 0, 0, 0)[::2]):
         with pytest.raises(ValueError, match="marks"):
             paged.PagedCache(c.k, c.v, c.table, c.lengths, c.refs, c.status, bad)
+
+
+def rows_of(c, r, n):
+    """Keys and values of the first n tokens of row r."""
+    t = torch.arange(n, device="cuda")
+    page = c.table[r][t // c.page_size].long()
+    return c.k[:, page, t % c.page_size].clone(), c.v[:, page, t % c.page_size].clone()
+
+
+@pytest.mark.parametrize("page_size,length", [(4, 6), (4, 1), (7, 13), (16, 20)])
+def test_a_row_adopted_into_a_page_does_not_write_there(cuda, page_size, length):
+    """Adopted, extended and appended to: the donor's tokens stay, and the donor
+    goes on in its page; a fork of the row goes on behind what it adopted."""
+    held = -(-length // page_size)
+    c = make(n_pages=20, rows=8, width=6, page_size=page_size)
+    c.extend(ints(0), ints(held * page_size - 1))            # its last page has a place left
+    c.adopt(ints(1, 2), c.table[:1, :held].expand(2, held), ints(length, length))
+    c.fork(ints(1), ints(3))
+    before = c.k.clone(), c.v.clone()
+    for step in range(held * page_size - length):            # up to the page's end
+        c.extend(ints(1, 2), ints(1, 1))
+        append_everywhere(c, ints(1, 2))
+        append_everywhere(c, ints(1), ints(length + step))   # nor by index
+    untouched(c, before)
+    with pytest.raises(RuntimeError, match="place"):
+        c.check()
+    c.extend(ints(0), ints(1))
+    append_everywhere(c, ints(0))
+    last = [(int(c.table[0, held - 1]), page_size - 1)]
+    untouched(c, before, last)
+    c.extend(ints(1), ints(1))                               # a page of its own again
+    append_everywhere(c, ints(1))
+    untouched(c, before, last + [(int(c.table[1, held]), 0)])
+    c.extend(ints(3), ints(1))                               # a fork: at once
+    append_everywhere(c, ints(3))
+    assert int(c.table[3, length // page_size]) != int(c.table[1, length // page_size])
+    untouched(c, before, last + [(int(c.table[1, held]), 0), (int(c.table[3, length // page_size]), length % page_size)])
+    assert all(torch.equal(a, b) for a, b in zip(rows_of(c, 3, length), rows_of(c, 0, length)))
+    c.check()
+
+
+@pytest.mark.parametrize("length,window", [(21, 0), (21, 9), (5, 0), (700, 0)])
+@pytest.mark.parametrize("copies", [1, 40, 1100])
+def test_the_rest_of_an_adopted_page_is_not_attended_to(cuda, length, window, copies):
+    """The same result before the row grows past its adopted tokens, with and
+    without a fork, as after it, wherever the donor's later tokens are: they are
+    NaN here."""
+    page_size, dim = 16, 64
+    held = -(-length // page_size)
+    c = paged.PagedCache.allocate(1, 200, page_size, 2, dim, 6, max(held + 3, 110))
+    g = torch.Generator(device="cuda").manual_seed(length)
+    c.extend(ints(0, 5), ints(held * page_size, 1700))
+    c.k.normal_(generator=g), c.v.normal_(generator=g)
+    page, slot = int(c.table[0, held - 1]), length % page_size
+    c.k[:, page, slot:], c.v[:, page, slot:] = float("nan"), float("nan")
+    c.adopt(ints(1), c.table[:1, :held], ints(length))
+    q = torch.randn(1, 4, dim, generator=g, device="cuda").half().expand(copies + 1, 4, dim)
+    rows = torch.full((copies + 1,), 1, dtype=torch.int32, device="cuda")
+    rows[copies // 2] = 5                                    # a longer row among them
+    at = torch.arange(copies + 1, device="cuda") != copies // 2
+
+    def attend(r):
+        out = c.attend(0, q, torch.where(rows == 1, r, rows).int(), return_lse=True, window=window)
+        assert all(t[at].isfinite().all() for t in out)
+        assert all(torch.equal(t[at], t[at][:1].expand_as(t[at])) for t in out if copies < 1000)
+        return [t[at][0] for t in out]
+
+    plain = attend(1)
+    more = held * page_size - length
+    c.extend(ints(1), ints(more))                            # to the page's end: nothing there is the row's
+    if not window:
+        assert all(torch.equal(a, b) for a, b in zip(attend(1), plain))
+    c.fork(ints(1), ints(2))                                 # nor is it the fork's
+    assert int(c.marks[2]) == length
+    if not window:
+        assert all(torch.equal(a, b) for a, b in zip(attend(2), plain))
+    # behind the page the row goes on; it and its fork attend to the same
+    c.extend(ints(1), ints(3))
+    kv = torch.randn(3, 2, dim, generator=g, device="cuda").half()
+    three = held * page_size + torch.arange(3, dtype=torch.int32, device="cuda")
+    c.append(0, kv, kv, ints(1, 1, 1), three)
+    c.fork(ints(1), ints(3))
+    grown = attend(1)
+    assert all(torch.equal(a, b) for a, b in zip(attend(3), grown))
+    # the same tokens in pages that the row holds whole
+    c.extend(ints(4), ints(length + 3))
+    t = torch.arange(length + 3, device="cuda")
+    source = torch.where(t < length, t, t - length + held * page_size)
+    from_page, to_page = c.table[1][source // page_size].long(), c.table[4][t // page_size].long()
+    for cache in (c.k, c.v):
+        cache[:, to_page, t % page_size] = cache[:, from_page, source % page_size]
+    if not window:
+        for a, b in zip(attend(4), grown):                   # tokens in other tiles: other rounding
+            assert (a.float() - b.float()).abs().max() <= 2 ** -9 * (1 + b.float().abs().max())
+    c.check()
+
+
+def test_an_emptied_row_forgets_where_it_was_adopted(cuda):
+    c = make(n_pages=8, rows=4, width=4)
+    c.extend(ints(0), ints(8))
+    c.adopt(ints(1), c.table[:1, :2], ints(6))
+    assert c.marks.tolist() == [0, 6, 0, 0]
+    c.extend(ints(1), ints(1))
+    assert c.marks.tolist() == [0, 6, 0, 0]
+    c.extend(ints(1), ints(100))                             # refused
+    assert c.marks[1] < 0
+    c.fork(ints(1), ints(2))
+    assert c.marks[1] == c.marks[2]
+    c.free(ints(1, 2))
+    c.adopt(ints(1), c.table[:1, :2], ints(4))               # whole pages, if fewer
+    assert c.marks.tolist() == [0, 0, 0, 0]
+    c.free(ints(1))
+    c.marks[1] = 6
+    c.extend(ints(1), ints(7))
+    assert c.marks.tolist() == [0, 0, 0, 0]
+    before = c.k.clone(), c.v.clone()
+    append_everywhere(c, ints(1))
+    untouched(c, before, [(int(c.table[1, 1]), 2)])

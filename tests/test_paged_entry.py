@@ -19,3 +19,8 @@ def test_a_rows_last_token_needs_marks():
     with pytest.raises(ValueError, match="marks"):
         _lib.call("jb_kv_append", cache(), 0, 1, None, 0, 0, None, 0, 0, 0, 4096, 0, 0, 4096, 0, 0, 4096, None, None,
                   0, None, 0, 1.0, 0, None)
+
+
+def test_adopting_part_of_a_page_needs_marks():
+    with pytest.raises(ValueError, match="marks"):
+        _lib.call("jb_pages_adopt", cache(), 4096, 4096, 4, 4, 4096, 1, None)
