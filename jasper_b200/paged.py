@@ -27,6 +27,7 @@ import ctypes as C
 import math
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _lib
 
@@ -107,29 +108,46 @@ class Rotary:
         """``x`` [tokens, heads, head_dim] or [batch, tokens, heads, head_dim]
         (float16, bfloat16 or float32; any strides with contiguous heads)
         turned by ``positions`` (int32 or int64, [tokens] or [batch, tokens]).
-        ``out`` may be ``x``.  Differentiable in ``x`` unless ``out`` is given."""
-        if out is None and x.requires_grad and torch.is_grad_enabled():
-            return _Turn.apply(x, positions, self)
-        return _lib.paged_module().rotary(x, positions, out, False, *self._args)
+        ``out`` may be ``x``.  Differentiable in ``x``, any number of times and
+        in forward mode too, unless ``out`` is given."""
+        return self._turn(x, positions, out, False)
 
     __call__ = apply
 
     def grad(self, dy: torch.Tensor, positions: torch.Tensor,
              out: torch.Tensor | None = None) -> torch.Tensor:
-        """The gradient with respect to apply()'s ``x``, given its output's."""
-        return _lib.paged_module().rotary(dy, positions, out, True, *self._args)
+        """The gradient with respect to apply()'s ``x``, given its output's;
+        differentiable in ``dy`` as apply() is in ``x``."""
+        return self._turn(dy, positions, out, True)
+
+    def _turn(self, x, positions, out, inverse):
+        if out is None and (x.requires_grad and torch.is_grad_enabled()
+                            or forward_ad.unpack_dual(x).tangent is not None):
+            return _Turn.apply(x, positions, self, inverse)
+        return _lib.paged_module().rotary(x, positions, out, inverse, *self._args)
 
 
 class _Turn(torch.autograd.Function):
+    """A turn is linear in x, and its transpose is the turn backwards: each is
+    the other's gradient, and its own forward derivative."""
+
     @staticmethod
-    def forward(ctx, x, positions, rotary):
-        ctx.rotary = rotary
+    def forward(x, positions, rotary, inverse):
+        return _lib.paged_module().rotary(x, positions, None, inverse, *rotary._args)
+
+    @staticmethod
+    def setup_context(ctx, inputs, output):
+        _, positions, ctx.rotary, ctx.inverse = inputs
         ctx.save_for_backward(positions)
-        return _lib.paged_module().rotary(x, positions, None, False, *rotary._args)
+        ctx.save_for_forward(positions)
 
     @staticmethod
     def backward(ctx, dy):
-        return ctx.rotary.grad(dy, ctx.saved_tensors[0]), None, None
+        return ctx.rotary._turn(dy, ctx.saved_tensors[0], None, not ctx.inverse), None, None, None
+
+    @staticmethod
+    def jvp(ctx, dx, *_):
+        return ctx.rotary._turn(dx, ctx.saved_tensors[0], None, ctx.inverse)
 
 
 class PagedCache:
