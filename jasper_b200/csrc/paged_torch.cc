@@ -10,6 +10,7 @@
 #include <Python.h>
 
 #include <ATen/ATen.h>
+#include <ATen/core/grad_mode.h>
 #include <ATen/cuda/EmptyTensor.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
@@ -157,6 +158,13 @@ void check_out(const Tensor& out, const Tensor& like, const char* name) {
   if (out.sizes() != like.sizes() || out.scalar_type() != like.scalar_type() ||
       out.device() != like.device() || (out.stride(-1) != 1 && out.size(-1) != 1))
     refuse(name, " must have the input's shape, type and device, and contiguous heads");
+  if ((out.requires_grad() && at::GradMode::is_enabled()) || out._fw_grad(0).defined())
+    refuse(name, " must not require a gradient: what is written to it is not recorded");
+}
+
+// A tensor of the caller's was written to: autograd sees that by its version.
+void written(const Tensor& t) {
+  if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
 }
 
 Tensor empty(at::IntArrayRef sizes, at::ScalarType type, c10::Device dev) {
@@ -209,6 +217,7 @@ PyObject* py_rotary(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
                         uint32_t(dim), uint32_t(integer(a[6])), pos.const_data_ptr(),
                         pos.scalar_type() == at::kLong, static_cast<const int64_t*>(freq.const_data_ptr()),
                         float(real(a[7])), truth(a[8]), truth(a[3]), stream_of(dev.index())));
+    if (a[2] != Py_None) written(out);
     return THPVariable_Wrap(out);
   });
 }
@@ -258,6 +267,7 @@ PyObject* py_append(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
         turn ? uint32_t(integer(a[11])) : 0, turn ? float(real(a[12])) : 1.0f, turn && truth(a[13]),
         stream_of(c.device)));
     if (!has_q) Py_RETURN_NONE;
+    if (a[8] != Py_None) written(q_out);
     return THPVariable_Wrap(q_out);
   });
 }
@@ -303,6 +313,7 @@ PyObject* py_attend(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
                            uint32_t(window), float(scale),
                            return_lse ? static_cast<float*>(lse.mutable_data_ptr()) : nullptr,
                            stream_of(c.device)));
+    if (a[8] != Py_None) written(out);
     if (!return_lse) return THPVariable_Wrap(out);
     PyObject *o = THPVariable_Wrap(out), *l = THPVariable_Wrap(lse);
     PyObject* pair = o && l ? PyTuple_Pack(2, o, l) : nullptr;

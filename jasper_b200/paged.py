@@ -109,7 +109,8 @@ class Rotary:
         (float16, bfloat16 or float32; any strides with contiguous heads)
         turned by ``positions`` (int32 or int64, [tokens] or [batch, tokens]).
         ``out`` may be ``x``.  Differentiable in ``x``, any number of times and
-        in forward mode too, unless ``out`` is given."""
+        in forward mode too, unless ``out`` (which must not require a gradient)
+        is given."""
         return self._turn(x, positions, out, False)
 
     __call__ = apply
