@@ -14,9 +14,12 @@
 #include <ATen/cuda/EmptyTensor.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
+#include <torch/csrc/autograd/functions/basic_ops.h>
+#include <torch/csrc/autograd/functions/utils.h>
 #include <torch/csrc/autograd/python_variable.h>
 
 #include <cmath>
+#include <memory>
 #include <sstream>
 #include <stdexcept>
 #include <string>
@@ -167,6 +170,19 @@ void written(const Tensor& t) {
   if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
 }
 
+// A call without derivatives: its results, made from q, raise in a backward pass
+// that reaches them, and tangents are refused.
+void check_tangent(const Tensor& q, const char* call) {
+  if (q._fw_grad(0).defined()) refuse(call, " has no forward-mode derivative");
+}
+template <typename... R>
+void not_differentiable(const char* call, const Tensor& q, const R&... results) {
+  if (!torch::autograd::compute_requires_grad(q)) return;
+  const std::shared_ptr<torch::autograd::Node> fn(
+      new torch::autograd::NotImplemented(call, torch::autograd::collect_next_edges(q)), torch::autograd::deleteNode);
+  (torch::autograd::set_history(results, fn), ...);
+}
+
 Tensor empty(at::IntArrayRef sizes, at::ScalarType type, c10::Device dev) {
   return at::detail::empty_cuda(sizes, type, dev, std::nullopt);
 }
@@ -247,6 +263,7 @@ PyObject* py_append(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
       if (!turn) refuse("q is only taken to be rotated: pass rotary");
       q = heads(tensor(a[6], "q"), "q", -1, c.head_dim, type, dev);
       if (q.size(0) != n) refuse("q must have ", n, " tokens, got ", q.size(0));
+      check_tangent(q, "PagedCache.append");
       if (a[8] != Py_None) {
         q_out = tensor(a[8], "q_out");
         check_out(q_out, q, "q_out");
@@ -268,6 +285,7 @@ PyObject* py_append(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
         stream_of(c.device)));
     if (!has_q) Py_RETURN_NONE;
     if (a[8] != Py_None) written(q_out);
+    else not_differentiable("PagedCache.append", q, q_out);
     return THPVariable_Wrap(q_out);
   });
 }
@@ -279,6 +297,7 @@ PyObject* py_attend(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
     const jb_page_cache& c = cache_at(a[0]);
     const c10::Device dev = device_of(c);
     Tensor q = heads(tensor(a[2], "q"), "q", -1, c.head_dim, type_of(c), dev);
+    check_tangent(q, "PagedCache.attend");
     const int64_t n = q.size(0), n_heads = q.size(1);
     if (n_heads % c.n_kv_heads)
       refuse("q's heads (", n_heads, ") must be a multiple of the cache's (", c.n_kv_heads, ")");
@@ -314,6 +333,8 @@ PyObject* py_attend(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
                            return_lse ? static_cast<float*>(lse.mutable_data_ptr()) : nullptr,
                            stream_of(c.device)));
     if (a[8] != Py_None) written(out);
+    else not_differentiable("PagedCache.attend", q, out);
+    if (return_lse) not_differentiable("PagedCache.attend", q, lse);
     if (!return_lse) return THPVariable_Wrap(out);
     PyObject *o = THPVariable_Wrap(out), *l = THPVariable_Wrap(lse);
     PyObject* pair = o && l ? PyTuple_Pack(2, o, l) : nullptr;

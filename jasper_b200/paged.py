@@ -19,7 +19,10 @@ Tensors are checked and passed on by a small CPython module
 include/jasper_b200.h).  Calls are asynchronous on torch's current stream of
 the cache's device and read nothing back: a row or page that does not fit sets
 a bit of the cache's status word, which :meth:`PagedCache.check` reads.  After
-a first call they can be captured into CUDA graphs.  No reference counterpart.
+a first call they can be captured into CUDA graphs.  The cache is for
+inference: a backward pass that reaches the results of append() or attend()
+raises, and none goes into the keys and values that it holds.  No reference
+counterpart.
 """
 from __future__ import annotations
 

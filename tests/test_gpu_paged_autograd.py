@@ -53,3 +53,25 @@ def test_outputs_that_require_a_gradient(cuda):
                 call(out)
         with forward_ad.dual_level(), pytest.raises(ValueError, match="gradient"):
             call(forward_ad.make_dual(leaf.detach(), torch.ones_like(leaf)))
+
+
+def test_a_backward_pass_through_the_cache_raises(cuda):
+    c, r = make()
+    q = torch.randn(2, 2, 8, device="cuda").half().requires_grad_()
+    kv = torch.randn(2, 1, 8, device="cuda").half()
+    for call in (lambda: c.append(0, kv, kv, ints(0, 1), q=q, rotary=r), lambda: c.attend(0, q),
+                 lambda: c.attend(0, q, return_lse=True)[0], lambda: c.attend(0, q, return_lse=True)[1],
+                 lambda: c.attend(0, (q * 2).transpose(0, 1)[:, :1].contiguous().transpose(0, 1))):
+        out = call()
+        with pytest.raises(RuntimeError, match="not implemented"):
+            (out.float().sum() + (q.float() ** 2).sum()).backward()
+        with torch.no_grad():
+            assert not call().requires_grad
+        q.requires_grad_(False)
+        assert torch.equal(call(), out) and not call().requires_grad
+        with forward_ad.dual_level():
+            plain, q = q, forward_ad.make_dual(q, torch.ones_like(q))
+            with pytest.raises(ValueError, match="forward-mode"):
+                call()
+            q = plain
+        q.requires_grad_()
