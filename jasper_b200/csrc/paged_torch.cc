@@ -299,7 +299,7 @@ PyObject* py_attend(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
     Tensor q = heads(tensor(a[2], "q"), "q", -1, c.head_dim, type_of(c), dev);
     check_tangent(q, "PagedCache.attend");
     const int64_t n = q.size(0), n_heads = q.size(1);
-    if (n_heads % c.n_kv_heads)
+    if (c.n_kv_heads && n_heads % c.n_kv_heads)  // a cache without heads is refused below, with its other limits
       refuse("q's heads (", n_heads, ") must be a multiple of the cache's (", c.n_kv_heads, ")");
     if (q.stride(0) % 8 || q.stride(1) % 8 || reinterpret_cast<uintptr_t>(q.const_data_ptr()) % 16)
       q = q.clone(at::MemoryFormat::Contiguous);
