@@ -28,6 +28,9 @@
 //  * A weight enters the second product as the sum of two 16-bit values (its
 //    rounding, and the rounding of what that left), so nothing is lost
 //    against float32 weights; l sums the float32 weights.
+//  * An infinite value times a weight's second half, or a weight that rounds to
+//    zero, would be NaN, so a result that is not finite is looked at again: what
+//    the values attended to hold in its place decides (settle()).
 //  * Short rows take no part in this: warps, blocks or clusters of blocks have
 //    a row's head each, and join in (distributed) shared memory.
 //
@@ -55,6 +58,7 @@ template <typename T>
 struct Mma;
 template <>
 struct Mma<__half> {
+  static constexpr uint32_t kExponent = 0x7C00;  // the bits of an infinity without its sign
   static __device__ __forceinline__ void mma(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
     asm(
         "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
@@ -73,6 +77,7 @@ struct Mma<__half> {
 };
 template <>
 struct Mma<__nv_bfloat16> {
+  static constexpr uint32_t kExponent = 0x7F80;
   static __device__ __forceinline__ void mma(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
     asm(
         "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
@@ -124,6 +129,10 @@ __device__ __forceinline__ float exp2_fast(float x) {
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
   return r;
 }
+
+// What a part's result adds to a sum, at a factor of 0 to 1: an infinity stays
+// one, however small the factor is.
+__device__ __forceinline__ float weighed(float x, float f) { return fabsf(x) == INFINITY ? x : x * f; }
 
 // Where the part results of a call lie: worker w has slot 2w for a row's head
 // that began before its part, slot 2w + 1 for one that goes on behind it.
@@ -481,6 +490,71 @@ struct Attend {
     }
   }
 
+  // Which elements of the values of c's row's head that are attended to in tiles
+  // `tile`, `tile` + `step` and so on below `end` are +inf, -inf or NaN: three
+  // bits for each of the 8 elements of chunk lane % kChunkLanes.  Not inlined:
+  // calls with finite values never get here.
+  static __device__ __noinline__ uint32_t odd_values(const AttendParams& p, Cursor c, int32_t end, int32_t step,
+                                                     int lane) {
+    const Lists none{};
+    const Attend self{p, none, lane};
+    const jb_page_cache& k = p.a.c;
+    const int chunk = lane % kChunkLanes, row0 = lane / kChunkLanes;
+    const bool inside = chunk < int(k.head_dim / 8);
+    const int64_t base = int64_t(p.a.layer) * k.layer_stride + int64_t(c.vh / p.head_tiles) * k.head_stride + chunk * 8;
+    uint32_t bits = 0;
+    for (; c.tile < end; c.tile += step) {
+      const Place x = self.place_of(c);
+      const bool there = uint32_t(x.page) < k.n_pages;
+      const uint32_t mask = __ballot_sync(kFullMask, x.seen && there) & 0xFFFFu;
+      const uint32_t slot = x.slot + (p.tiled_pages ? lane & 15 : 0);
+      const int64_t mine = there ? x.page * k.page_stride + slot * k.token_stride : 0;
+      for (int row = row0; row < TK; row += kRowsPerCopy) {
+        const int64_t off = __shfl_sync(kFullMask, mine, row) + base;
+        if (!inside || !((mask >> row) & 1)) continue;
+        const uint4 v = *reinterpret_cast<const uint4*>(static_cast<const T*>(k.v) + off);
+        const uint32_t word[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+        for (int e = 0; e < 8; e++) {
+          const uint32_t b = (word[e / 2] >> (16 * (e % 2))) & 0xFFFFu;
+          if ((b & Mma<T>::kExponent) == Mma<T>::kExponent)
+            bits |= ((b & 0x7FFFu) != Mma<T>::kExponent ? 4u : b >> 15 ? 2u : 1u) << (3 * e);
+        }
+      }
+    }
+#pragma unroll
+    for (int d = kChunkLanes; d < 32; d <<= 1) bits |= __shfl_xor_sync(kFullMask, bits, d);
+    return bits;
+  }
+
+  // Behind tiles `tile`, `tile` + `step` and so on below `end`: a result that is
+  // not finite is what the values attended to make it, infinite if they are
+  // infinite with one sign, however small the weights.  One that is not finite
+  // for another reason (a NaN score, an overflow) stays.
+  __device__ __forceinline__ void settle(State& s, const Cursor& c, int32_t tile, int32_t end, int32_t step) const {
+    float odd = 0.0f;  // NaN if a result is infinite or NaN
+#pragma unroll
+    for (int n = 0; n < NT; n++)
+#pragma unroll
+      for (int k = 0; k < KS; k++)
+#pragma unroll
+        for (int j = 0; j < 4; j++) odd = fmaf(s.o[n][k][j], 0.0f, odd);
+    if (!__any_sync(kFullMask, odd != 0.0f)) return;
+    Cursor from = c;
+    from.tile = tile;
+    const uint32_t bits = odd_values(p, from, end, step, lane);
+#pragma unroll
+    for (int k = 0; k < KS; k++)
+#pragma unroll
+      for (int j = 0; j < 4; j += 2) {
+        const uint32_t b = (__shfl_sync(kFullMask, bits, 2 * k + j / 2) >> (3 * (lane / 4))) & 7;
+        if (b == 0) continue;
+        const float v = b == 1 ? INFINITY : b == 2 ? -INFINITY : NAN;
+#pragma unroll
+        for (int n = 0; n < NT; n++) s.o[n][k][j] = s.o[n][k][j + 1] = v;
+      }
+  }
+
   // The piece's end: the result, or a part of it (slot >= 0).
   __device__ __forceinline__ void finish(State& s, uint32_t i, uint32_t vh, int64_t slot) const {
 #pragma unroll
@@ -578,6 +652,7 @@ struct Attend {
     State s;
     begin(s, c.i, c.vh);
     bool whole = c.tile == c.t.begin;
+    int32_t piece = c.tile;  // the piece's first tile
     int stage = 0;
     for (;;) {
       copies_wait<STAGES - 2>();
@@ -591,6 +666,7 @@ struct Attend {
       const bool ends = c.tile + 1 == c.t.end;
       if (ends || left == 0) {
         const int64_t slot_of = ends ? (whole ? -1 : 2 * int64_t(worker)) : whole ? 2 * int64_t(worker) + 1 : 2 * int64_t(worker);
+        settle(s, c, piece, c.tile + 1, 1);
         finish(s, c.i, c.vh, slot_of);
         if (whole && lane == 0 && (!ends || !p.by_worker)) {
           int parts = 0;
@@ -607,6 +683,7 @@ struct Attend {
         next(c);
         begin(s, c.i, c.vh);
         whole = true;
+        piece = c.tile;
       } else {
         c.tile++;
       }
@@ -754,6 +831,7 @@ __global__ void __launch_bounds__(WARPS * 32) attend_cluster_kernel(const __grid
     }
     copies_wait<0>();
     __syncwarp();
+    self.settle(s, c, c.t.begin + first, c.t.end, step);
   }
   if (blocks == 1 && each == 1) {  // the warp has it all
     if (has) self.finish(s, c.i, c.vh, -1);
@@ -815,10 +893,10 @@ __global__ void __launch_bounds__(WARPS * 32) attend_cluster_kernel(const __grid
       const float f = warp_f[w][column];
       const float4 x = *reinterpret_cast<const float4*>(
           reinterpret_cast<const float*>(smem + w * STAGES * A::kStageBytes) + column * OS + d);
-      o.x += x.x * f;
-      o.y += x.y * f;
-      o.z += x.z * f;
-      o.w += x.w * f;
+      o.x += weighed(x.x, f);
+      o.y += weighed(x.y, f);
+      o.z += weighed(x.z, f);
+      o.w += weighed(x.w, f);
     }
     if (blocks == 1) put(column, d, group_rl[group][column].x, o, group_rl[group][column].y);
     else *reinterpret_cast<float4*>(&block_o[column][d]) = o;
@@ -853,10 +931,10 @@ __global__ void __launch_bounds__(WARPS * 32) attend_cluster_kernel(const __grid
 #pragma unroll
     for (int b = 0; b < kCluster; b++) {
       const float f = exp2_fast(rl[b].x - r);
-      o.x += part[b].x * f;
-      o.y += part[b].y * f;
-      o.z += part[b].z * f;
-      o.w += part[b].w * f;
+      o.x += weighed(part[b].x, f);
+      o.y += weighed(part[b].y, f);
+      o.z += weighed(part[b].z, f);
+      o.w += weighed(part[b].w, f);
       l += rl[b].y * f;
     }
     put(column, d, ref, o, l);
@@ -912,13 +990,13 @@ __global__ void __launch_bounds__(join_warps(SHARED) * 32) join_kernel(const __g
     const float keep = exp2_fast(ref - r);
     l *= keep;
 #pragma unroll
-    for (int k = 0; k < N; k++) o[k] *= keep;
+    for (int k = 0; k < N; k++) o[k] = weighed(o[k], keep);
 #pragma unroll
     for (int b = 0; b < B; b++) {
       const float f = exp2_fast(rl[b].x - r);
       l += rl[b].y * f;
 #pragma unroll
-      for (int k = 0; k < N; k++) o[k] += part[b][k] * f;
+      for (int k = 0; k < N; k++) o[k] += weighed(part[b][k], f);
     }
     ref = top;
   }
@@ -946,7 +1024,7 @@ __global__ void __launch_bounds__(join_warps(SHARED) * 32) join_kernel(const __g
 #pragma unroll
       for (int i = 0; i < SHARED; i++) {
         const float f = exp2_fast(share_rl[i].x - r);
-        v += share[i][d] * f;
+        v += weighed(share[i][d], f);
         l += share_rl[i].y * f;
       }
       out[d] = Mma<T>::from(l == 0.0f ? 0.0f : v / l);
