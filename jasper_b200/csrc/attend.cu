@@ -49,16 +49,20 @@ namespace {
 constexpr uint32_t kFullMask = 0xFFFFFFFFu;
 constexpr int kMaxListed = 1024;  // queries whose lengths a block keeps in shared memory
 constexpr int TK = 16;            // tokens of a tile
-// A weight is 2^(s - r): r is set 6 below the largest score and stays until a
-// score is 15 above it, so weights reach 2^15, inside float16, and the largest
-// is at least 2^6: float16 weights keep 24 + 6 bits below the largest.
-constexpr float kRefBelow = 6.0f, kRefRoom = 15.0f;
+// A weight is 2^(s - r): r is set kRefBelow below the largest score and stays
+// until a score is kRefRoom above it.  In float16 weights reach 2^15, inside its
+// range, and the largest is at least 2^6, so they keep 24 + 6 bits below the
+// largest.  bfloat16 has float32's range, for weights and for values, and a sum
+// of large values with weights above 1 would overflow: there r lies 8 above the
+// largest score, weights are at most 1, and hundreds of tokens of equal weight
+// with values near the end of the range still have a finite sum.
 
 template <typename T>
 struct Mma;
 template <>
 struct Mma<__half> {
   static constexpr uint32_t kExponent = 0x7C00;  // the bits of an infinity without its sign
+  static constexpr float kRefBelow = 6.0f, kRefRoom = 15.0f;
   static __device__ __forceinline__ void mma(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
     asm(
         "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
@@ -78,6 +82,7 @@ struct Mma<__half> {
 template <>
 struct Mma<__nv_bfloat16> {
   static constexpr uint32_t kExponent = 0x7F80;
+  static constexpr float kRefBelow = -8.0f, kRefRoom = 0.0f;
   static __device__ __forceinline__ void mma(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
     asm(
         "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
@@ -438,7 +443,7 @@ struct Attend {
 #pragma unroll
       for (int j = 0; j < 4; j++) {
         w[n][j] = (j < 2 ? seen0 : seen1) ? w[n][j] * scale : -INFINITY;
-        far |= w[n][j] > s.ref[n][j & 1] + kRefRoom;
+        far |= w[n][j] > s.ref[n][j & 1] + Mma<T>::kRefRoom;
       }
     if (__any_sync(kFullMask, far)) {
 #pragma unroll
@@ -448,7 +453,7 @@ struct Attend {
           float top = fmaxf(w[n][j], w[n][j + 2]);
 #pragma unroll
           for (int d = 4; d < 32; d <<= 1) top = fmaxf(top, __shfl_xor_sync(kFullMask, top, d));
-          const float ref = fmaxf(s.ref[n][j], top - kRefBelow);
+          const float ref = fmaxf(s.ref[n][j], top - Mma<T>::kRefBelow);
           const float keep = s.ref[n][j] == -INFINITY ? 0.0f : exp2_fast(s.ref[n][j] - ref);
           s.ref[n][j] = ref;
           s.sum[n][j] *= keep;
