@@ -216,12 +216,11 @@ PyObject* py_rotary(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
     }
     flat_out = out;
     if (x.dim() == 4) {
-      if (out.size(0) > 1 && out.size(1) > 0 && out.stride(0) != out.size(1) * out.stride(1))
-        refuse("out's batch and tokens must be one run of tokens");
       if (pos.dim() < 1 || pos.dim() > 2 || pos.size(-1) != x.size(1) || (pos.dim() == 2 && pos.size(0) != x.size(0)))
         refuse("positions must be [", x.size(0), ", ", x.size(1), "] or [", x.size(1), "], got ", pos.sizes());
       pos = pos.expand({x.size(0), x.size(1)}).reshape({-1});
       flat_out = out.flatten(0, 1);
+      if (flat_out.const_data_ptr() != out.const_data_ptr()) refuse("out's batch and tokens must be one run of tokens");
       x = x.flatten(0, 1);
     }
     const int64_t dim = integer(a[5]);
