@@ -394,7 +394,9 @@ typedef struct jb_page_cache {
  * (i, i + rot_dim / 2), or (2i, 2i + 1) with `interleaved`.  freq[i] (device,
  * rot_dim / 2 values) is pair i's turn for one position in units of 2^-64 of
  * a turn: products with whole positions wrap at whole turns, so angles are
- * exact to float32 for every int64 position.  `inverse` turns backwards: the
+ * reduced exactly for every int64 position; freq's own rounding is all that
+ * grows with it, by at most 2^-65 of a turn a position, which is a float32
+ * angle's rounding at 2^39.  `inverse` turns backwards: the
  * gradient with respect to x, given y's.  x and y: [n_tokens][n_heads]
  * [head_dim] of `dtype` at any token and head stride (elements), head_dim at
  * most 512; y may be x.

@@ -5,8 +5,9 @@
 //     s (a cos t - b sin t),  s (b cos t + a sin t),   t = p theta_i,
 // and the gradient is the same turn backwards.  theta_i comes as a fraction
 // of a turn in 64-bit fixed point: p * freq wraps at whole turns, so the top
-// 32 bits of the product are the reduced angle, exact for every int64
-// position; only then does it become a float32 (error 2^-25 of a turn).
+// 32 bits of the product are the reduced angle, exact for that theta and every
+// int64 position; only then does it become a float32 (error 2^-26 of a turn, to
+// which theta's rounding adds up to 2^-65 of a turn a position).
 //
 // HBM bounds prompts, latency single tokens.  A block takes a few tokens: it
 // computes their cosines and sines once (half a head of pairs each, shared by

@@ -27,6 +27,7 @@ counterpart.
 from __future__ import annotations
 
 import ctypes as C
+import decimal
 import math
 
 import torch
@@ -37,6 +38,9 @@ from . import _lib
 __all__ = ["Rotary", "PagedCache"]
 
 _DTYPES = {torch.float16: 0, torch.bfloat16: 1, torch.float32: 2}
+
+_PI = decimal.Decimal("3.14159265358979323846264338327950288419716939937510582097494459")
+_DIGITS = decimal.Context(prec=40)  # of frequencies, on their way to 64-bit fixed point
 
 EXHAUSTED, BAD_ROW, BAD_TOKEN = 1, 2, 4
 _STATUS = {
@@ -61,8 +65,10 @@ class Rotary:
     turn more than ``beta_fast`` times, blends between, and multiplies the
     rotated elements by 0.1 ln(factor) + 1.
 
-    Thetas are kept as 64-bit fixed-point fractions of a turn, so angles are
-    reduced exactly: positions may be any int32 or int64.
+    Thetas are kept as 64-bit fixed-point fractions of a turn, rounded once to
+    their last unit, so angles are reduced exactly and are off by at most
+    2^-65 of a turn a position: no more than a float32 angle's own rounding for
+    positions up to 2^39, and known for every int32 or int64.
     """
 
     def __init__(self, head_dim: int, rot_dim: int | None = None, *, base: float = 10000.0,
@@ -86,21 +92,27 @@ class Rotary:
             raise ValueError("scaling 'yarn' needs trained_length")
         self.head_dim, self.rot_dim, self.layout = head_dim, rot_dim, layout
         self.scale = 1.0
-        if scaling == "ntk":
-            base = base * factor ** (rot_dim / (rot_dim - 2))
-        theta = [base ** (-2.0 * i / rot_dim) for i in range(rot_dim // 2)]
-        if scaling == "linear":
-            theta = [t / factor for t in theta]
-        elif scaling == "yarn":
-            def pair_of(turns):  # the pair that turns so often over the trained length
-                return rot_dim * math.log(trained_length / (turns * 2 * math.pi)) / (2 * math.log(base))
-            low = max(math.floor(pair_of(beta_fast)), 0)
-            high = min(math.ceil(pair_of(beta_slow)), rot_dim - 1)
-            slow = [min(1.0, max(0.0, (i - low) / max(high - low, 0.001))) for i in range(len(theta))]
-            theta = [t / factor * s + t * (1 - s) for t, s in zip(theta, slow)]
-            self.scale = 0.1 * math.log(factor) + 1.0
-        self.theta = theta
-        turns = [round(t / (2 * math.pi) * 2.0 ** 64) % 2 ** 64 for t in theta]
+        with decimal.localcontext(_DIGITS):
+            wide, by = decimal.Decimal(float(base)), decimal.Decimal(float(factor))
+            if scaling == "ntk":
+                wide *= by ** (decimal.Decimal(rot_dim) / (rot_dim - 2))
+            step, theta = wide ** (decimal.Decimal(-2) / rot_dim), [decimal.Decimal(1)]
+            for _ in range(rot_dim // 2 - 1):
+                theta.append(theta[-1] * step)
+            if scaling == "linear":
+                theta = [t / by for t in theta]
+            elif scaling == "yarn":
+                def pair_of(turns):  # the pair that turns so often over the trained length
+                    return rot_dim * math.log(trained_length / (turns * 2 * math.pi)) / (2 * math.log(base))
+                low = max(math.floor(pair_of(beta_fast)), 0)
+                high = min(math.ceil(pair_of(beta_slow)), rot_dim - 1)
+                ramp = max(decimal.Decimal(high - low), decimal.Decimal("0.001"))
+                slow = [min(1, max(0, (i - low) / ramp)) for i in range(len(theta))]
+                theta = [t / by * s + t * (1 - s) for t, s in zip(theta, slow)]
+                self.scale = 0.1 * math.log(factor) + 1.0
+            radian = 2 ** 64 / (2 * _PI)
+            turns = [int((t * radian).to_integral_value()) % 2 ** 64 for t in theta]
+        self.theta = [float(t) for t in theta]
         self._freq = torch.tensor([t - 2 ** 64 if t >= 2 ** 63 else t for t in turns],
                                   dtype=torch.int64).to(device)
         self.device = self._freq.device
