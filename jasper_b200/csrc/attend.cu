@@ -26,8 +26,10 @@
 //    shared by warps, and the weights through tensor memory and back; the
 //    tensor pipe is 15 % busy here, so it has nothing to give.
 //  * A weight enters the second product as the sum of two 16-bit values (its
-//    rounding, and the rounding of what that left), so nothing is lost
-//    against float32 weights; l sums the float32 weights.
+//    rounding, and the rounding of what that left), which carry it to 2^-17 of
+//    itself in bfloat16, 2^-23 in float16.  The result is rounded to 2^-8 and
+//    2^-11 of itself once, 500 times as much or more; one 16-bit value would
+//    have cost as much as that rounding.  l sums the float32 weights.
 //  * An infinite value times a weight's second half, or a weight that rounds to
 //    zero, would be NaN, so a result that is not finite is looked at again: what
 //    the values attended to hold in its place decides (settle()).
@@ -35,8 +37,9 @@
 //    a row's head each, and join in (distributed) shared memory.
 //
 // Measured: 64 rows of 1 to 8191 tokens, 8 heads of 128, bfloat16, 167 us, 6.4
-// TB/s (0.99 of the measured copy rate); 400 k + 333 k tokens, float16, 442 us,
-// 6.8 TB/s; one row of 1000 tokens 5.9 us.
+// TB/s (0.99 of the measured copy rate); 400 k + 333 k tokens, float16, 446 us,
+// 6.7 TB/s; one row of 1000 tokens 5.7 us in a table of its width, 9.4 in one of
+// 16,000 tokens or more.
 #include <cmath>
 #include <mutex>
 #include <stdexcept>
@@ -51,11 +54,14 @@ constexpr int kMaxListed = 1024;  // queries whose lengths a block keeps in shar
 constexpr int TK = 16;            // tokens of a tile
 // A weight is 2^(s - r): r is set kRefBelow below the largest score and stays
 // until a score is kRefRoom above it.  In float16 weights reach 2^15, inside its
-// range, and the largest is at least 2^6, so they keep 24 + 6 bits below the
-// largest.  bfloat16 has float32's range, for weights and for values, and a sum
-// of large values with weights above 1 would overflow: there r lies 8 above the
-// largest score, weights are at most 1, and hundreds of tokens of equal weight
-// with values near the end of the range still have a finite sum.
+// range, and the largest is at least 2^6, so that a weight that float16 drops is
+// below 2^-31 of the largest in the same worker's part: 2^18 of them, a part of a
+// batch of 4 10^8 tokens, weigh less than half the result's rounding.  (12 below
+// and room of 3 would drop 64 times less, for 1.4 % of the time of two long rows
+// and 3 % of 1000 short ones.)  bfloat16 has float32's range, for weights and for
+// values, and a sum of large values with weights above 1 would overflow: there r
+// lies 8 above the largest score, weights are at most 1, and hundreds of tokens of
+// equal weight with values near the end of the range still have a finite sum.
 
 template <typename T>
 struct Mma;
@@ -190,7 +196,7 @@ __device__ __forceinline__ Tiles tiles_of(const AttendArgs& a, uint32_t i) {
   return t;
 }
 
-// Inclusive sum over the block's threads (256 at most) of one value each.
+// Inclusive sum over the block's THREADS threads of one value each.
 template <int THREADS>
 __device__ __forceinline__ int64_t block_sum_scan(int64_t v, int64_t* total) {
   __shared__ int64_t sums[THREADS / 32];
@@ -1074,13 +1080,15 @@ Shape shape_of(const AttendArgs& a) {
   s.warps = ring_of(s.dp, s.nt).warps;
   s.workers = uint32_t(sm_count() * s.warps);
   s.row_heads = uint64_t(a.n) * a.c.n_kv_heads * s.head_tiles;
-  // Clusters as large as all run at once (15 of 8 blocks take 7 us, 16 take
-  // 13; 33 and 36 of 4, 7.8 and 13.4), where rows are short enough, by the
-  // table's width or the window, that unequal lengths cost less than the
-  // second kernel.  Clusters / equal parts, heads of 128: one row of 1000
-  // tokens and 8 heads 6.4 / 10.0 us, of 8000 14.0 / 14.0; 32 rows' heads of
-  // 4000 tokens 18 / 21, of 1000 to 4000 14 / 15; 64 of 4000 28 / 31, of 1000
-  // to 4000 26 / 24.
+  // For 148 SMs: clusters as large as all run at once (15 of 8 blocks take 7 us,
+  // 16 take 13; 33 and 36 of 4, 7.8 and 13.4), where rows are short enough that
+  // unequal lengths cost less than the second kernel.  How long they are is
+  // known here by the table's width or the window only: in a wide table short
+  // rows take the equal parts too (20 rows of 50 tokens, 8 heads: 4.9 us in a
+  // table of 64 tokens, 11.2 in one of 16,000).  Clusters / equal parts, heads
+  // of 128: one row of 1000 tokens and 8 heads 6.4 / 10.0 us, of 8000 14.0 /
+  // 14.0; 32 rows' heads of 4000 tokens 18 / 21, of 1000 to 4000 14 / 15; 64 of
+  // 4000 28 / 31, of 1000 to 4000 26 / 24.
   const uint64_t wide = uint64_t(a.c.max_pages) * a.c.page_size;
   const uint64_t longest = a.window && a.window < wide ? a.window : wide;
   s.cluster = s.row_heads <= 15 ? 8 : s.row_heads <= 32 ? 4 : s.row_heads <= 74 ? 2 : 1;

@@ -624,7 +624,7 @@ void launch_copies(CopyArgs a, cudaStream_t st) {
   a.by_head = c.token_stride == dim;
   a.flat = token_rows || (a.by_head && a.tokens == nullptr && c.head_stride == ps * dim);
   const uint64_t full = uint64_t(c.page_size) * c.n_kv_heads * (c.head_dim / 8);
-  constexpr uint64_t kMost = 148 * 8;
+  constexpr uint64_t kMost = 148 * 8;  // blocks: 8 an SM
   const uint64_t pieces = (full + 32 * kCopyDepth - 1) / (32 * kCopyDepth);
   uint64_t units = uint64_t(a.n) * 2 * c.n_layers * pieces;
   a.run = uint32_t(units / (kMost * (kCopyThreads / 32) * 2));  // two units at least for every warp
