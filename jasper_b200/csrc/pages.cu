@@ -381,9 +381,10 @@ fork_kernel(const jb_page_cache c, const int32_t* parents, const int32_t* childr
       c.lengths[w.row[i]] = len;
       // A refused parent's last token is an old one in its child too.  Where
       // the parent ends as it was adopted, the child's last page is its own.
-      // A parent that is another pair's child is empty, whatever its mark.
+      // An empty parent may be another pair's child: its mark is not read.
       if (c.marks) {
-        const int32_t mark = i == threadIdx.x ? first.mark : c.marks[parents[i]], adopted = mark & kMarkAdopted;
+        const int32_t mark = len == 0 ? 0 : i == threadIdx.x ? first.mark : c.marks[parents[i]];
+        const int32_t adopted = mark & kMarkAdopted;
         c.marks[w.row[i]] = (mark & kMarkRefused) | (len > adopted ? adopted : 0);
       }
     } else if (len >= 0) {

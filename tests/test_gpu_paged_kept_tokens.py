@@ -250,3 +250,16 @@ def test_an_emptied_row_forgets_where_it_was_adopted(cuda):
     before = c.k.clone(), c.v.clone()
     append_everywhere(c, ints(1))
     untouched(c, before, [(int(c.table[1, 1]), 2)])
+
+
+def test_forks_of_empty_rows_carry_no_mark(cuda):
+    """A chain of pairs, each child the next one's parent: all but the first
+    parent are empty, and only its child is a copy of a refused row."""
+    n = 2500
+    c = make(n_pages=2, rows=n + 1, width=1, page_size=2, layers=1)
+    c.extend(ints(0), ints(2))
+    every = torch.arange(n + 1, dtype=torch.int32, device="cuda")
+    c.extend(every, torch.full_like(every, 3))               # no row has place for so many
+    assert (c.marks < 0).all() and c.lengths.sum() == 2
+    c.fork(every[:-1], every[1:])
+    assert c.lengths[:3].tolist() == [2, 2, 0] and (c.marks[:2] < 0).all() and (c.marks[2:] == 0).all()
