@@ -365,8 +365,8 @@ int jb_merge_topk_strided(const int32_t* shard_idx, const float* shard_dist, uin
  * the same for both; head_dim contiguous; every stride, and both bases, a
  * multiple of 16 bytes; head_dim a multiple of 8, at most 256).  A row (a
  * conversation) holds lengths[row] tokens in the pages table[row][0 ..
- * ceil(length / page_size)); an entry of -1 is a page that is not there: its
- * tokens are never attended to.  refs[page] counts the rows that hold a page;
+ * ceil(length / page_size)), and -1 in the entries behind them; an entry of -1
+ * is a page that is not there: its tokens are never attended to.  refs[page] counts the rows that hold a page;
  * 0 is free.  marks[row] has its sign set while the row's last jb_pages_extend
  * was refused: its last token is then an old one, and jb_kv_append without index
  * leaves it alone.  Its other bits are the length that jb_pages_adopt gave the
