@@ -38,7 +38,7 @@
 //
 // Measured: 64 rows of 1 to 8191 tokens, 8 heads of 128, bfloat16, 167 us, 6.4
 // TB/s (0.99 of the measured copy rate); 400 k + 333 k tokens, float16, 446 us,
-// 6.7 TB/s; one row of 1000 tokens 5.7 us in a table of its width, 9.4 in one of
+// 6.7 TB/s; one row of 1000 tokens 5.4 us in a table of its width, 9.3 in one of
 // 16,000 tokens or more.
 #include <cmath>
 #include <mutex>
@@ -173,14 +173,11 @@ struct AttendParams {
 // The tiles of TK tokens that query i reads.
 struct Tiles {
   int32_t row, len, first, begin, end;
-  uint32_t gap, gap_len;  // tokens that lie in the rest of a page in which the row was adopted: not its own
-  __device__ __forceinline__ void set_gap(const jb_page_cache& c, int32_t adopted) {
-    gap = uint32_t(adopted);
-    gap_len = adopted ? (c.page_size - gap % c.page_size) % c.page_size : 0;
-  }
+  uint32_t gap;  // where the row was adopted inside a page: from here on that page is not its own
 };
-__device__ __forceinline__ int32_t adopted_length(const jb_page_cache& c, int32_t row) {
-  return c.marks && row >= 0 && uint32_t(row) < c.n_rows ? c.marks[row] & kMarkAdopted : 0;
+__device__ __forceinline__ uint32_t gap_of(const jb_page_cache& c, int32_t row) {
+  const int32_t adopted = c.marks && row >= 0 && uint32_t(row) < c.n_rows ? c.marks[row] & kMarkAdopted : 0;
+  return adopted ? uint32_t(adopted) : 0xFFFFFFFFu;
 }
 __device__ __forceinline__ Tiles tiles_of(const AttendArgs& a, uint32_t i) {
   Tiles t;
@@ -192,7 +189,7 @@ __device__ __forceinline__ Tiles tiles_of(const AttendArgs& a, uint32_t i) {
   t.first = a.window && len > int64_t(a.window) ? int32_t(len - a.window) : 0;
   t.begin = t.first / TK;
   t.end = int32_t((len + TK - 1) / TK);
-  t.set_gap(a.c, adopted_length(a.c, t.row));
+  t.gap = gap_of(a.c, t.row);
   return t;
 }
 
@@ -294,7 +291,8 @@ struct Attend {
   static constexpr int kRowsPerCopy = 32 / kChunkLanes;
 
   struct Lists {
-    int32_t *row, *len, *adopted;
+    int32_t *row, *len;
+    uint32_t* gap;
     int64_t* prefix;
   };
 
@@ -310,7 +308,7 @@ struct Attend {
     t.first = p.a.window && t.len > int64_t(p.a.window) ? int32_t(t.len - p.a.window) : 0;
     t.begin = t.first / TK;
     t.end = int32_t((int64_t(t.len) + TK - 1) / TK);
-    t.set_gap(p.a.c, lists.adopted[i]);
+    t.gap = lists.gap[i];
     return t;
   }
   __device__ __forceinline__ uint32_t head_rows() const { return p.a.c.n_kv_heads * p.head_tiles; }
@@ -337,11 +335,12 @@ struct Attend {
   __device__ __forceinline__ Place place_of(const Cursor& c) const {
     Place x;
     const uint32_t t = uint32_t(c.tile) * TK + (lane & 15);
-    x.seen = int32_t(t) >= c.t.first && int32_t(t) < c.t.len && t - c.t.gap >= c.t.gap_len;
+    x.seen = int32_t(t) >= c.t.first && int32_t(t) < c.t.len;
     if (x.seen && p.a.mask && t < p.a.mask_width) x.seen = p.a.mask[int64_t(c.i) * p.a.mask_stride + t];
     const uint32_t at = p.tiled_pages ? uint32_t(c.tile) * TK : min(t, uint32_t(c.t.len) - 1);
     const uint32_t pg = at / p.a.c.page_size;
     x.slot = at - pg * p.a.c.page_size;
+    if (t >= c.t.gap && pg * p.a.c.page_size < c.t.gap) x.seen = false;
     x.page = p.a.c.table[c.t.row * p.a.c.table_stride + pg];
     return x;
   }
@@ -501,19 +500,46 @@ struct Attend {
     }
   }
 
-  // Which elements of the values of c's row's head that are attended to in tiles
-  // `tile`, `tile` + `step` and so on below `end` are +inf, -inf or NaN: three
-  // bits for each of the 8 elements of chunk lane % kChunkLanes.  Not inlined:
-  // calls with finite values never get here.
-  static __device__ __noinline__ uint32_t odd_values(const AttendParams& p, Cursor c, int32_t end, int32_t step,
-                                                     int lane) {
+  // Is a result of the warp's not finite?
+  __device__ __forceinline__ bool odd(const State& s) const {
+    float x[4] = {0.0f, 0.0f, 0.0f, 0.0f};  // NaN if one is infinite or NaN
+#pragma unroll
+    for (int n = 0; n < NT; n++)
+#pragma unroll
+      for (int k = 0; k < KS; k++)
+#pragma unroll
+        for (int j = 0; j < 4; j++) x[j] = fmaf(s.o[n][k][j], 0.0f, x[j]);
+    return __any_sync(kFullMask, (x[0] + x[1]) + (x[2] + x[3]) != 0.0f);
+  }
+
+  // The columns whose sums are NaN, as bits: theirs stay NaN.
+  __device__ __forceinline__ uint32_t nan_columns(const State& s) const {
+    uint32_t bits = 0;
+#pragma unroll
+    for (int n = 0; n < NT; n++)
+#pragma unroll
+      for (int j = 0; j < 2; j++) bits |= uint32_t(isnan(s.sum[n][j])) << (8 * n + 2 * (lane % 4) + j);
+    return __reduce_or_sync(kFullMask, bits);
+  }
+
+  // Behind finish(), where a result of query i's tiles `tile`, tile + step and so on
+  // below `end` was odd(): elements whose values that are attended to are infinite
+  // with one sign become that, however small the weights; with both, or with NaN,
+  // NaN.  What is not finite for another reason stays.  The results are at o
+  // (floats, `stride` to a column), or, if that is null, the call's output.  Calls
+  // with finite values never get here: it is not inlined, and looks up again what
+  // its callers would have to keep in registers.
+  static __device__ __noinline__ void settle(const AttendParams& p, uint32_t i, uint32_t vh, int32_t tile, int32_t end,
+                                             int32_t step, uint32_t nan_columns, float* o, int stride) {
     const Lists none{};
+    const int lane = int(threadIdx.x & 31);
     const Attend self{p, none, lane};
     const jb_page_cache& k = p.a.c;
+    Cursor c{tiles_of(p.a, i), i, vh, tile};
     const int chunk = lane % kChunkLanes, row0 = lane / kChunkLanes;
     const bool inside = chunk < int(k.head_dim / 8);
     const int64_t base = int64_t(p.a.layer) * k.layer_stride + int64_t(c.vh / p.head_tiles) * k.head_stride + chunk * 8;
-    uint32_t bits = 0;
+    uint32_t bits = 0;  // +inf, -inf, NaN for each of the 8 elements of the chunk
     for (; c.tile < end; c.tile += step) {
       const Place x = self.place_of(c);
       const bool there = uint32_t(x.page) < k.n_pages;
@@ -535,35 +561,23 @@ struct Attend {
     }
 #pragma unroll
     for (int d = kChunkLanes; d < 32; d <<= 1) bits |= __shfl_xor_sync(kFullMask, bits, d);
-    return bits;
-  }
-
-  // Behind tiles `tile`, `tile` + `step` and so on below `end`: a result that is
-  // not finite is what the values attended to make it, infinite if they are
-  // infinite with one sign, however small the weights.  One that is not finite
-  // for another reason (a NaN score, an overflow) stays.
-  __device__ __forceinline__ void settle(State& s, const Cursor& c, int32_t tile, int32_t end, int32_t step) const {
-    float odd = 0.0f;  // NaN if a result is infinite or NaN
-#pragma unroll
-    for (int n = 0; n < NT; n++)
-#pragma unroll
-      for (int k = 0; k < KS; k++)
-#pragma unroll
-        for (int j = 0; j < 4; j++) odd = fmaf(s.o[n][k][j], 0.0f, odd);
-    if (!__any_sync(kFullMask, odd != 0.0f)) return;
-    Cursor from = c;
-    from.tile = tile;
-    const uint32_t bits = odd_values(p, from, end, step, lane);
-#pragma unroll
-    for (int k = 0; k < KS; k++)
-#pragma unroll
-      for (int j = 0; j < 4; j += 2) {
-        const uint32_t b = (__shfl_sync(kFullMask, bits, 2 * k + j / 2) >> (3 * (lane / 4))) & 7;
-        if (b == 0) continue;
-        const float v = b == 1 ? INFINITY : b == 2 ? -INFINITY : NAN;
-#pragma unroll
-        for (int n = 0; n < NT; n++) s.o[n][k][j] = s.o[n][k][j + 1] = v;
-      }
+    // the lane's elements as finish() has them
+    for (int d8 = 0; d8 < DP / 8; d8++) {
+      const uint32_t b = (__shfl_sync(kFullMask, bits, d8) >> (3 * (lane / 4))) & 7;
+      const int d = 8 * d8 + lane / 4;
+      if (b == 0) continue;
+      const float v = b == 1 ? INFINITY : b == 2 ? -INFINITY : NAN;
+      for (int n = 0; n < NT; n++)
+        for (int j = 0; j < 2; j++) {
+          const int column = 8 * n + 2 * (lane % 4) + j;
+          if (!self.head_real(c.vh, column) || ((nan_columns >> column) & 1)) continue;
+          if (o)
+            o[column * stride + d] = v;
+          else
+            static_cast<T*>(p.a.out.p)[int64_t(c.i) * p.a.out.token_stride +
+                                       int64_t(self.head_of(c.vh, column)) * p.a.out.head_stride + d] = Mma<T>::from(v);
+        }
+    }
   }
 
   // The piece's end: the result, or a part of it (slot >= 0).
@@ -662,7 +676,6 @@ struct Attend {
 
     State s;
     begin(s, c.i, c.vh);
-    bool whole = c.tile == c.t.begin;
     int32_t piece = c.tile;  // the piece's first tile
     int stage = 0;
     for (;;) {
@@ -676,9 +689,13 @@ struct Attend {
       left--;
       const bool ends = c.tile + 1 == c.t.end;
       if (ends || left == 0) {
+        const bool whole = piece == c.t.begin;
         const int64_t slot_of = ends ? (whole ? -1 : 2 * int64_t(worker)) : whole ? 2 * int64_t(worker) + 1 : 2 * int64_t(worker);
-        settle(s, c, piece, c.tile + 1, 1);
+        const bool odd_results = odd(s);
         finish(s, c.i, c.vh, slot_of);
+        if (odd_results)
+          settle(p, c.i, c.vh, piece, c.tile + 1, 1, nan_columns(s),
+                 slot_of < 0 ? nullptr : p.parts.o + slot_of * kColumns * DP, DP);
         if (whole && lane == 0 && (!ends || !p.by_worker)) {
           int parts = 0;
           if (!ends) {  // the row's head goes on: in how many parts, this one included
@@ -693,7 +710,6 @@ struct Attend {
         if (left == 0) break;
         next(c);
         begin(s, c.i, c.vh);
-        whole = true;
         piece = c.tile;
       } else {
         c.tile++;
@@ -703,15 +719,24 @@ struct Attend {
   }
 };
 
+// Registers of a thread: 12 warps with 128 leave room on their SM for blocks of
+// the kernel that follows, which are launched early (32 rows of 500 to 4000
+// tokens, 8 heads of 128: 53.6 us, 55.7 with 166); 12 warps of 96 x 16 columns
+// need their 168, fewer warps take what there is.
+constexpr int registers_of(int DP, int NT) {
+  return ring_of(DP, NT).warps < 12 ? 255 : DP == 96 && NT == 2 ? 168 : 128;
+}
+
 template <typename T, int DP, int NT, int WARPS, int STAGES>
-__global__ void __launch_bounds__(WARPS * 32) attend_kernel(const __grid_constant__ AttendParams p) {
+__global__ void __maxnreg__(registers_of(DP, NT)) attend_kernel(const __grid_constant__ AttendParams p) {
   using A = Attend<T, DP, NT, WARPS, STAGES>;
   extern __shared__ __align__(1024) unsigned char smem[];
   uint32_t* valid = reinterpret_cast<uint32_t*>(smem + A::kRingBytes);
   int64_t* prefix = reinterpret_cast<int64_t*>(smem + ((A::kRingBytes + WARPS * STAGES * 4 + 7) & ~7));
   int32_t* row = reinterpret_cast<int32_t*>(prefix + kMaxListed + 1);
-  int32_t *len = row + kMaxListed, *adopted = len + kMaxListed;
-  typename A::Lists lists{row, len, adopted, prefix};
+  int32_t* len = row + kMaxListed;
+  uint32_t* gap = reinterpret_cast<uint32_t*>(len + kMaxListed);
+  typename A::Lists lists{row, len, gap, prefix};
   const int wid = threadIdx.x >> 5;
   A self{p, lists, int(threadIdx.x & 31)};
   follow();
@@ -729,7 +754,7 @@ __global__ void __launch_bounds__(WARPS * 32) attend_kernel(const __grid_constan
         const Tiles t = tiles_of(p.a, i);
         row[i] = t.row;
         len[i] = t.len;
-        adopted[i] = adopted_length(p.a.c, t.row);
+        gap[i] = t.gap;
         v = max(t.end - t.begin, 0);
       }
       int64_t sum;
@@ -842,10 +867,11 @@ __global__ void __launch_bounds__(WARPS * 32) attend_cluster_kernel(const __grid
     }
     copies_wait<0>();
     __syncwarp();
-    self.settle(s, c, c.t.begin + first, c.t.end, step);
   }
+  const bool odd_results = first < count && self.odd(s);
   if (blocks == 1 && each == 1) {  // the warp has it all
     if (has) self.finish(s, c.i, c.vh, -1);
+    if (odd_results) A::settle(p, c.i, c.vh, c.t.begin + first, c.t.end, step, self.nan_columns(s), nullptr, 0);
     return;
   }
   if (first < count) {
@@ -866,6 +892,7 @@ __global__ void __launch_bounds__(WARPS * 32) attend_cluster_kernel(const __grid
           o[column * OS + 16 * k + lane / 4 + 8] = s.o[n][k][j + 2];
         }
       }
+    if (odd_results) A::settle(p, c.i, c.vh, c.t.begin + first, c.t.end, step, self.nan_columns(s), o, OS);
   }
   __syncthreads();
   const int warp0 = group * each, t = int(threadIdx.x) - warp0 * 32;
@@ -1084,8 +1111,8 @@ Shape shape_of(const AttendArgs& a) {
   // 16 take 13; 33 and 36 of 4, 7.8 and 13.4), where rows are short enough that
   // unequal lengths cost less than the second kernel.  How long they are is
   // known here by the table's width or the window only: in a wide table short
-  // rows take the equal parts too (20 rows of 50 tokens, 8 heads: 4.9 us in a
-  // table of 64 tokens, 11.2 in one of 16,000).  Clusters / equal parts, heads
+  // rows take the equal parts too (20 rows of 50 tokens, 8 heads: 4.5 us in a
+  // table of 64 tokens, 10.7 in one of 16,000).  Clusters / equal parts, heads
   // of 128: one row of 1000 tokens and 8 heads 6.4 / 10.0 us, of 8000 14.0 /
   // 14.0; 32 rows' heads of 4000 tokens 18 / 21, of 1000 to 4000 14 / 15; 64 of
   // 4000 28 / 31, of 1000 to 4000 26 / 24.
